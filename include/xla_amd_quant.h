@@ -34,6 +34,11 @@ extern "C" {
 #define XLA_AMD_TARGET_DEQUANT_DOT "xla_amd.dequant_dot"
 #define XLA_AMD_TARGET_FP8_SCALED_DOT "xla_amd.fp8_scaled_dot"
 #define XLA_AMD_TARGET_QUANTIZE_FP8 "xla_amd.rowwise_quantize_fp8"
+/* custom_call_target strings of the 8-bit paged key/value cache; a module names them itself */
+#define XLA_AMD_TARGET_KV_CACHE_WRITE "xla_amd.kv_cache_write"
+#define XLA_AMD_TARGET_KV_CACHE_ATTENTION "xla_amd.kv_cache_attention"
+#define XLA_AMD_TARGET_KV_CACHE_PAGES "xla_amd.kv_cache_pages"
+#define XLA_AMD_TARGET_KV_CACHE_COPY_PAGES "xla_amd.kv_cache_copy_pages"
 
 /* ------------------------------------------------------------------------
  * Layer 1: XLA FFI handlers (stage EXECUTE; they also answer the metadata
@@ -130,7 +135,88 @@ XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_fp8_scaled_dot(XLA_FFI_CallFrame* call_fra
 XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_rowwise_quantize_fp8(XLA_FFI_CallFrame* call_frame);
 
 /*
- * Registers the three handlers above for platform "ROCM" through the table's
+ * The 8-bit paged key/value cache of a decoder.  A layer's cache is a pool of `pages` pages of `page`
+ * tokens: codes S8 or F8E4M3FN [pages, kv_heads, page, head] for the keys and the same for the values, and
+ * F32 scales [pages, kv_heads, page / block], one for each block of `block` tokens and head; a cached value is
+ * code * scale.  page and block are powers of two, page is 16 to 1024, block divides page, head is a multiple
+ * of 16 up to 256.  Position t of sequence b lies in page page_table[b, t / page] at row t % page.  The
+ * rows of a call lie behind each other: sequence b owns rows [q_offsets[b], q_offsets[b+1]), which are the
+ * last ones of its kv_lens[b] positions; rows from q_offsets[batch] on belong to nobody.  Tables, lengths and
+ * offsets are read on the device only.  What they hold cannot make a call reach outside its buffers:
+ * offsets are clamped to the rows, lengths to the table, and a position whose page lies outside
+ * [0, pages) is neither read nor written.
+ *
+ * kv_cache_write quantises new rows into the pages.  For every block it touches, and each head:
+ *   amax = max |x| over the block's new rows;  s = amax / 127 (S8) or amax / 448 (F8E4M3FN);
+ *   if the block held rows of the sequence before: s = max(s, old scale), and every code c it held becomes
+ *     convert(clamp(c * (old scale / s)));
+ *   code = convert(clamp(x / s)), 0 where the quotient is no number or s is 0;  scale = s.
+ *   All operations are f32, each rounded once; convert rounds to nearest, ties to even.  A NaN in x makes s
+ *   NaN (and with it the block's values); no NaN code is ever stored.
+ *   args: k, v BF16 [rows, kv_heads, head]; k_cache, v_cache; k_scales, v_scales; page_table S32 [batch, width];
+ *         kv_lens S32 [batch] (with the new rows); q_offsets S32 [batch + 1]
+ *   rets: k_cache, v_cache, k_scales, v_scales, the operands' own buffers (output_to_operand_aliasing)
+ *   No two positions that a call writes may lie in one page row, and no block that it touches may belong to
+ *   two sequences (XLA_AMD_TARGET_KV_CACHE_PAGES never shares a page that is not full).
+ */
+XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_kv_cache_write(XLA_FFI_CallFrame* call_frame);
+
+/*
+ * Softmax attention of the rows of a call over the cache.  Row i of the n rows of sequence b stands at
+ * position p = kv_lens[b] - n + i and sees position j if j < kv_lens[b], and j <= p (causal), and
+ * j > p - window (window > 0).  Head h of q reads cache head h / (q_heads / kv_heads).
+ *   x_j = softmax_scale * (q . k_j), with softcap > 0: softcap * tanh(x_j / softcap);
+ *   out = sum_j exp(x_j) v_j / sum_j exp(x_j);  lse = log sum_j exp(x_j)
+ *   A row that sees nothing, or belongs to nobody, is 0 and its lse -infinity.
+ *   Sums, maxima and the softmax are f32; the weights exp(x_j) times the scale of v_j are rounded to bf16 on
+ *   their way into the matrix instruction.
+ *   args: q BF16 [rows, q_heads, head]; k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets
+ *   rets: out BF16 [rows, q_heads, head]; optionally lse F32 [rows, q_heads]; optionally scratch S8 or U8 (what
+ *         xla_amd_kv_cache_attention_workspace_bytes says; without it the keys of a sequence are not split
+ *         over workgroups)
+ *   attrs: softmax_scale f32 (default 1 / sqrt(head)); causal pred (default true); window i64 (default 0: none;
+ *          needs causal); softcap f32 (default 0: none)
+ *   F8E4M3FN codes are taken to be numbers (kv_cache_write stores no others); positions that no row of a call
+ *   sees may hold anything.
+ */
+XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_kv_cache_attention(XLA_FFI_CallFrame* call_frame);
+
+/*
+ * Book-keeping of the page pool.  State: page_table S32 [batch, width], kv_lens S32 [batch], ref_counts S32
+ * [pages] (0: free).  A sequence holds the first ceil(kv_lens / page_size) entries of its row; the others of the
+ * result are -1.  The call writes a new state next to the old one.  op:
+ *   RESERVE  request S32 [batch], wanted lengths.  A sequence whose request is below its length or above
+ *            width * page_size is refused.  Further pages are given, lowest free page first, in the order of the
+ *            sequences; once one does not fit, none behind it that needs a page gets one either.
+ *            status S32 [batch] is 1 where the length was granted.
+ *   FORK     request S32 [n, 2] of (source, destination).  The destination must be empty and not be named by an
+ *            earlier pair, the two must differ.  It shares the source's full pages; for a last page that is
+ *            not full it gets a free page of its own, and moves S32 [n, 2] lists (old page, new page) for
+ *            XLA_AMD_TARGET_KV_CACHE_COPY_PAGES, -1 behind the last.  Free pages go as above.  All pairs see the
+ *            old state.  status S32 [n].
+ *   FREE     request S32 [n] of sequences, whose pages lose a reference.  status S32 [n] is 0 for a number outside
+ *            the batch and for one named before.
+ *   COMPACT  no request.  With U pages in use, the pages in use from U on move, in order, into the free ones
+ *            below U, in order; moves S32 [pages / 2, 2] lists them, -1 behind the last; status S32 [0].
+ *   args: page_table, kv_lens, ref_counts [, request]
+ *   rets: page_table, kv_lens, ref_counts (buffers other than the operands'), moves S32 [m, 2] (m = 0 for RESERVE and
+ *         FREE), status, scratch S8 or U8 (xla_amd_kv_cache_pages_workspace_bytes; needed)
+ *   attrs: op string; page_size i64
+ *   Entries outside [0, pages) keep their value and count for nothing.
+ */
+XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_kv_cache_pages(XLA_FFI_CallFrame* call_frame);
+
+/*
+ * Copies whole pages inside every buffer of a pool: for each (source, destination) of moves,
+ * buffer[destination] = buffer[source].  Pairs that name a page outside [0, pages) are skipped.  No
+ * destination may occur twice or be a source too.
+ *   args: moves S32 [m, 2]; 1 to XLA_AMD_KV_CACHE_MAX_BUFFERS buffers of any type [pages, ...]
+ *   rets: the buffers, the operands' own (output_to_operand_aliasing)
+ */
+XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_kv_cache_copy_pages(XLA_FFI_CallFrame* call_frame);
+
+/*
+ * Registers the handlers above for platform "ROCM" through the table's
  * XLA_FFI_Handler_Register (xla/ffi/ffi_api.cc:280-315) -- the dynamic
  * counterpart of XLA_FFI_REGISTER_HANDLER.  Returns NULL or the first error.
  */
@@ -292,6 +378,90 @@ typedef struct XlaAmdRowwiseQuantize {
 } XlaAmdRowwiseQuantize;
 
 XLA_AMD_EXPORT int xla_amd_launch_rowwise_quantize_fp8(const XlaAmdRowwiseQuantize* p, void* stream);
+
+/* One layer's cache and the rows of a call (see xla_amd_kv_cache_write). */
+typedef struct XlaAmdKvCache {
+  void* k_cache; /* S8 or F8E4M3FN codes [pages, kv_heads, page_size, head_size], 16-byte aligned */
+  void* v_cache;
+  float* k_scales; /* [pages, kv_heads, page_size / block] */
+  float* v_scales;
+  const int32_t* page_table; /* [batch, table_width] */
+  const int32_t* kv_lens;    /* [batch] */
+  const int32_t* q_offsets;  /* [batch + 1] */
+  int64_t pages, kv_heads, page_size, head_size, block;
+  int64_t batch, table_width, rows;
+  int32_t cache_dtype; /* S8 or F8E4M3FN */
+  int32_t reserved0;
+} XlaAmdKvCache;
+
+typedef struct XlaAmdKvCacheWrite {
+  XlaAmdKvCache cache;
+  const void* k; /* bf16 [rows, kv_heads, head_size], 16-byte aligned */
+  const void* v;
+} XlaAmdKvCacheWrite;
+
+XLA_AMD_EXPORT int xla_amd_launch_kv_cache_write(const XlaAmdKvCacheWrite* p, void* stream);
+
+typedef struct XlaAmdKvCacheAttention {
+  XlaAmdKvCache cache;
+  const void* q; /* bf16 [rows, q_heads, head_size], 16-byte aligned */
+  void* out;     /* bf16 [rows, q_heads, head_size], 16-byte aligned */
+  float* lse;    /* [rows, q_heads] or NULL */
+  void* workspace; /* optional scratch, 16-byte aligned */
+  size_t workspace_bytes;
+  int64_t q_heads;
+  int64_t window; /* 0: none */
+  float softmax_scale;
+  float softcap; /* 0: none */
+  int32_t causal;
+  int32_t reserved0;
+} XlaAmdKvCacheAttention;
+
+XLA_AMD_EXPORT int xla_amd_launch_kv_cache_attention(const XlaAmdKvCacheAttention* p, void* stream);
+
+/* Scratch with which the keys of a sequence can be split over workgroups (f32 partial sums of at most
+ * as many pieces as the device holds workgroups; 0: the shape is never split). */
+XLA_AMD_EXPORT size_t xla_amd_kv_cache_attention_workspace_bytes(int64_t rows, int64_t batch, int64_t q_heads,
+                                                                 int64_t kv_heads, int64_t head_size,
+                                                                 int64_t max_positions);
+
+enum {
+  XLA_AMD_KV_PAGES_RESERVE = 0,
+  XLA_AMD_KV_PAGES_FORK = 1,
+  XLA_AMD_KV_PAGES_FREE = 2,
+  XLA_AMD_KV_PAGES_COMPACT = 3
+};
+
+typedef struct XlaAmdKvCachePages {
+  const int32_t* page_table; /* [batch, table_width] */
+  const int32_t* kv_lens;    /* [batch] */
+  const int32_t* ref_counts; /* [pages] */
+  const int32_t* request;    /* [batch], [n, 2] or [n]; NULL for COMPACT */
+  int32_t* page_table_out;   /* the new state, in buffers of its own */
+  int32_t* kv_lens_out;
+  int32_t* ref_counts_out;
+  int32_t* moves;  /* FORK [n, 2], COMPACT [pages / 2, 2], else unused */
+  int32_t* status; /* RESERVE [batch], FORK and FREE [n], COMPACT unused */
+  void* workspace; /* xla_amd_kv_cache_pages_workspace_bytes, 16-byte aligned */
+  size_t workspace_bytes;
+  int64_t batch, table_width, pages, page_size, requests; /* requests: n of FORK and FREE */
+  int32_t op; /* XLA_AMD_KV_PAGES_* */
+  int32_t reserved0;
+} XlaAmdKvCachePages;
+
+XLA_AMD_EXPORT int xla_amd_launch_kv_cache_pages(const XlaAmdKvCachePages* p, void* stream);
+XLA_AMD_EXPORT size_t xla_amd_kv_cache_pages_workspace_bytes(int64_t batch, int64_t pages, int64_t requests);
+
+#define XLA_AMD_KV_CACHE_MAX_BUFFERS 64
+
+typedef struct XlaAmdKvCacheCopyPages {
+  const int32_t* moves; /* [num_moves, 2] */
+  void* const* buffers; /* host array of num_buffers device pointers */
+  const int64_t* page_bytes; /* host array: bytes of one page of each buffer */
+  int64_t num_moves, pages, num_buffers;
+} XlaAmdKvCacheCopyPages;
+
+XLA_AMD_EXPORT int xla_amd_launch_kv_cache_copy_pages(const XlaAmdKvCacheCopyPages* p, void* stream);
 
 /* Message of the last failed launcher call on this thread ("" if none). */
 XLA_AMD_EXPORT const char* xla_amd_last_error(void);

@@ -79,6 +79,35 @@ int xla_amd_launch_rowwise_quantize_fp8(const XlaAmdRowwiseQuantize* p, void* st
   return xla_amd::LaunchRowwiseQuantize(*p, (hipStream_t)stream, xla_amd::GetOption("quantize_variant"));
 }
 
+int xla_amd_launch_kv_cache_write(const XlaAmdKvCacheWrite* p, void* stream) {
+  if (!p) return xla_amd::Fail(XLA_FFI_Error_Code_INVALID_ARGUMENT, "kv_cache_write: null params");
+  return xla_amd::LaunchKvCacheWrite(*p, (hipStream_t)stream);
+}
+
+int xla_amd_launch_kv_cache_attention(const XlaAmdKvCacheAttention* p, void* stream) {
+  if (!p) return xla_amd::Fail(XLA_FFI_Error_Code_INVALID_ARGUMENT, "kv_cache_attention: null params");
+  return xla_amd::LaunchKvCacheAttention(*p, (hipStream_t)stream);
+}
+
+int xla_amd_launch_kv_cache_pages(const XlaAmdKvCachePages* p, void* stream) {
+  if (!p) return xla_amd::Fail(XLA_FFI_Error_Code_INVALID_ARGUMENT, "kv_cache_pages: null params");
+  return xla_amd::LaunchKvCachePages(*p, (hipStream_t)stream);
+}
+
+int xla_amd_launch_kv_cache_copy_pages(const XlaAmdKvCacheCopyPages* p, void* stream) {
+  if (!p) return xla_amd::Fail(XLA_FFI_Error_Code_INVALID_ARGUMENT, "kv_cache_copy_pages: null params");
+  return xla_amd::LaunchKvCacheCopyPages(*p, (hipStream_t)stream);
+}
+
+size_t xla_amd_kv_cache_attention_workspace_bytes(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads,
+                                                  int64_t head_size, int64_t max_positions) {
+  return xla_amd::KvCacheAttentionWorkspaceBytes(rows, batch, q_heads, kv_heads, head_size, max_positions);
+}
+
+size_t xla_amd_kv_cache_pages_workspace_bytes(int64_t batch, int64_t pages, int64_t requests) {
+  return xla_amd::KvCachePagesWorkspaceBytes(batch, pages, requests);
+}
+
 size_t xla_amd_dequant_dot_workspace_bytes(int64_t batch, int64_t M, int64_t K, int64_t N,
                                            int32_t weight_dtype) {
   const size_t decode = xla_amd::DequantDotDecodeWorkspaceBytes(

@@ -327,6 +327,73 @@ int64_t Elements(const XLA_FFI_Buffer* b) {
   return n;
 }
 
+bool SameShape(const XLA_FFI_Buffer* a, const XLA_FFI_Buffer* b) {
+  if (a->rank != b->rank) return false;
+  for (int64_t i = 0; i < a->rank; ++i)
+    if (a->dims[i] != b->dims[i]) return false;
+  return true;
+}
+
+// Types whose values fill whole bytes, and how many.
+constexpr uint64_t kWholeByteMask =
+    Bit(XLA_FFI_DataType_PRED) | Bit(XLA_FFI_DataType_S8) | Bit(XLA_FFI_DataType_U8) | Bit(XLA_FFI_DataType_F8E4M3FN) |
+    Bit(XLA_FFI_DataType_F8E5M2) | Bit(XLA_FFI_DataType_S16) | Bit(XLA_FFI_DataType_U16) | Bit(XLA_FFI_DataType_F16) |
+    Bit(XLA_FFI_DataType_BF16) | Bit(XLA_FFI_DataType_S32) | Bit(XLA_FFI_DataType_U32) | Bit(XLA_FFI_DataType_F32);
+int64_t ElementBytes(int d) {
+  switch (d) {
+    case XLA_FFI_DataType_S16: case XLA_FFI_DataType_U16: case XLA_FFI_DataType_F16: case XLA_FFI_DataType_BF16: return 2;
+    case XLA_FFI_DataType_S32: case XLA_FFI_DataType_U32: case XLA_FFI_DataType_F32: return 4;
+    default: return 1;
+  }
+}
+
+// The operands that the calls over an 8-bit paged cache share, in this order: k_cache, v_cache, k_scales,
+// v_scales, page_table, kv_lens, q_offsets.
+constexpr uint64_t kCacheMask = Bit(XLA_FFI_DataType_S8) | Bit(XLA_FFI_DataType_F8E4M3FN);
+struct CacheOperands {
+  XLA_FFI_Buffer* buffers[4];
+  XLA_FFI_Buffer *table, *lens, *offsets;
+
+  void Decode(Decoder& d, int at) {
+    buffers[0] = d.Arg(at, kCacheMask, 4, 4, "k_cache");
+    buffers[1] = d.Arg(at + 1, kCacheMask, 4, 4, "v_cache");
+    buffers[2] = d.Arg(at + 2, Bit(XLA_FFI_DataType_F32), 3, 3, "k_scales");
+    buffers[3] = d.Arg(at + 3, Bit(XLA_FFI_DataType_F32), 3, 3, "v_scales");
+    table = d.Arg(at + 4, Bit(XLA_FFI_DataType_S32), 2, 2, "page_table");
+    lens = d.Arg(at + 5, Bit(XLA_FFI_DataType_S32), 1, 1, "kv_lens");
+    offsets = d.Arg(at + 6, Bit(XLA_FFI_DataType_S32), 1, 1, "q_offsets");
+  }
+  // What is wrong with their shapes, or nothing and *c filled (the launcher checks the sizes themselves).
+  std::string Check(int64_t rows, XlaAmdKvCache* c) const {
+    const int64_t* k = buffers[0]->dims;
+    const int64_t* s = buffers[2]->dims;
+    if (!SameShape(buffers[0], buffers[1]) || buffers[0]->dtype != buffers[1]->dtype)
+      return "k_cache and v_cache must have one shape and type";
+    if (!SameShape(buffers[2], buffers[3])) return "k_scales and v_scales must have one shape";
+    if (s[0] != k[0] || s[1] != k[1] || s[2] <= 0 || k[2] % s[2] != 0)
+      return "scales must be [pages,kv_heads,page/block]";
+    if (lens->dims[0] != table->dims[0]) return "kv_lens must have one entry per row of page_table";
+    if (offsets->dims[0] != table->dims[0] + 1) return "q_offsets must have one entry more than kv_lens";
+    c->k_cache = buffers[0]->data;
+    c->v_cache = buffers[1]->data;
+    c->k_scales = (float*)buffers[2]->data;
+    c->v_scales = (float*)buffers[3]->data;
+    c->page_table = (const int32_t*)table->data;
+    c->kv_lens = (const int32_t*)lens->data;
+    c->q_offsets = (const int32_t*)offsets->data;
+    c->pages = k[0];
+    c->kv_heads = k[1];
+    c->page_size = k[2];
+    c->head_size = k[3];
+    c->block = k[2] / s[2];
+    c->batch = table->dims[0];
+    c->table_width = table->dims[1];
+    c->rows = rows;
+    c->cache_dtype = buffers[0]->dtype;
+    return "";
+  }
+};
+
 struct CommonAttrs {
   int epilogue = XLA_AMD_EPI_DEFAULT;
   int32_t dequant_type = XLA_FFI_DataType_F32;
@@ -633,11 +700,190 @@ XLA_FFI_Error* xla_amd_rowwise_quantize_fp8(XLA_FFI_CallFrame* f) {
   return LaunchStatus(f, xla_amd_launch_rowwise_quantize_fp8(&p, stream));
 }
 
+XLA_FFI_Error* xla_amd_kv_cache_write(XLA_FFI_CallFrame* f) {
+  XLA_FFI_Error* err;
+  if (Preamble(f, 9, 9, 4, 4, &err)) return err;
+  Decoder d{f};
+  XLA_FFI_Buffer* k = d.Arg(0, Bit(XLA_FFI_DataType_BF16), 3, 3, "k");
+  XLA_FFI_Buffer* v = d.Arg(1, Bit(XLA_FFI_DataType_BF16), 3, 3, "v");
+  CacheOperands c;
+  c.Decode(d, 2);
+  XLA_FFI_Buffer* ret[4];
+  for (int i = 0; i < 4; ++i)
+    ret[i] = i < 2 ? d.Ret(i, kCacheMask, 4, 4, i ? "v_cache" : "k_cache")
+                   : d.Ret(i, Bit(XLA_FFI_DataType_F32), 3, 3, i == 3 ? "v_scales" : "k_scales");
+  if (!d.ok()) return d.Error();
+  XlaAmdKvCacheWrite p{};
+  std::string why = c.Check(k->dims[0], &p.cache);
+  if (why.empty()) {
+    if (k->dims[1] != p.cache.kv_heads || k->dims[2] != p.cache.head_size || !SameShape(k, v))
+      why = "k and v must be [rows,kv_heads,head]";
+    for (int i = 0; i < 4 && why.empty(); ++i)
+      if (!SameShape(ret[i], c.buffers[i]) || ret[i]->dtype != c.buffers[i]->dtype || ret[i]->data != c.buffers[i]->data)
+        why = "the results are the cache operands' own buffers (output_to_operand_aliasing)";
+  }
+  if (!why.empty()) return InvalidArgument(f->api, "xla_amd.kv_cache_write: " + why);
+  p.k = k->data;
+  p.v = v->data;
+  void* stream;
+  if (XLA_FFI_Error* e = GetStream(f, &stream)) return e;
+  return LaunchStatus(f, xla_amd_launch_kv_cache_write(&p, stream));
+}
+
+XLA_FFI_Error* xla_amd_kv_cache_attention(XLA_FFI_CallFrame* f) {
+  XLA_FFI_Error* err;
+  if (Preamble(f, 8, 8, 1, 3, &err)) return err;
+  Decoder d{f};
+  XLA_FFI_Buffer* q = d.Arg(0, Bit(XLA_FFI_DataType_BF16), 3, 3, "q");
+  CacheOperands c;
+  c.Decode(d, 1);
+  XLA_FFI_Buffer* out = d.Ret(0, Bit(XLA_FFI_DataType_BF16), 3, 3, "out");
+  // after out: an f32 matrix is the lse, a byte vector is scratch
+  XLA_FFI_Buffer* lse = nullptr;
+  XLA_FFI_Buffer* ws = nullptr;
+  for (int64_t i = 1; i < f->rets.size; ++i) {
+    const bool f32 = f->rets.types[i] == XLA_FFI_RetType_BUFFER &&
+                     static_cast<XLA_FFI_Buffer*>(f->rets.rets[i])->dtype == XLA_FFI_DataType_F32;
+    if (f32 && !lse && !ws) lse = d.Ret((int)i, Bit(XLA_FFI_DataType_F32), 2, 2, "lse");
+    else if (!ws) ws = d.Ret((int)i, kBytesMask, 1, 1, "scratch");
+    else return InvalidArgument(f->api, "xla_amd.kv_cache_attention: results are out[, lse][, scratch]");
+  }
+  XlaAmdKvCacheAttention p{};
+  bool causal = true;
+  float scale = 0.0f, softcap = 0.0f;
+  const bool has_scale = d.Scalar("softmax_scale", XLA_FFI_DataType_F32, &scale, 4);
+  d.Scalar("causal", XLA_FFI_DataType_PRED, &causal, 1);
+  d.Int("window", &p.window);
+  d.Scalar("softcap", XLA_FFI_DataType_F32, &softcap, 4);
+  if (!d.ok()) return d.Error();
+  std::string why = c.Check(q->dims[0], &p.cache);
+  if (why.empty()) {
+    if (q->dims[2] != p.cache.head_size || q->dims[1] <= 0 || q->dims[1] % p.cache.kv_heads != 0)
+      why = "q must be [rows,q_heads,head] with q_heads a multiple of kv_heads";
+    else if (!SameShape(out, q)) why = "out must have the shape of q";
+    else if (lse && (lse->dims[0] != q->dims[0] || lse->dims[1] != q->dims[1])) why = "lse must be [rows,q_heads]";
+  }
+  if (!why.empty()) return InvalidArgument(f->api, "xla_amd.kv_cache_attention: " + why);
+  p.q = q->data;
+  p.out = out->data;
+  p.lse = lse ? (float*)lse->data : nullptr;
+  p.workspace = ws ? ws->data : nullptr;
+  p.workspace_bytes = ws ? (size_t)Elements(ws) : 0;
+  p.q_heads = q->dims[1];
+  p.softmax_scale = has_scale ? scale : 1.0f / __builtin_sqrtf((float)p.cache.head_size);
+  p.softcap = softcap;
+  p.causal = causal ? 1 : 0;
+  void* stream;
+  if (XLA_FFI_Error* e = GetStream(f, &stream)) return e;
+  return LaunchStatus(f, xla_amd_launch_kv_cache_attention(&p, stream));
+}
+
+XLA_FFI_Error* xla_amd_kv_cache_pages(XLA_FFI_CallFrame* f) {
+  XLA_FFI_Error* err;
+  if (Preamble(f, 3, 4, 6, 6, &err)) return err;
+  Decoder d{f};
+  const uint64_t s32 = Bit(XLA_FFI_DataType_S32);
+  XLA_FFI_Buffer* tab = d.Arg(0, s32, 2, 2, "page_table");
+  XLA_FFI_Buffer* lens = d.Arg(1, s32, 1, 1, "kv_lens");
+  XLA_FFI_Buffer* refs = d.Arg(2, s32, 1, 1, "ref_counts");
+  XLA_FFI_Buffer* req = f->args.size > 3 ? d.Arg(3, s32, 1, 2, "request") : nullptr;
+  XLA_FFI_Buffer* tab_o = d.Ret(0, s32, 2, 2, "page_table");
+  XLA_FFI_Buffer* lens_o = d.Ret(1, s32, 1, 1, "kv_lens");
+  XLA_FFI_Buffer* refs_o = d.Ret(2, s32, 1, 1, "ref_counts");
+  XLA_FFI_Buffer* moves = d.Ret(3, s32, 2, 2, "moves");
+  XLA_FFI_Buffer* status = d.Ret(4, s32, 1, 1, "status");
+  XLA_FFI_Buffer* ws = d.Ret(5, kBytesMask, 1, 1, "scratch");
+  std::string op;
+  XlaAmdKvCachePages p{};
+  d.String("op", &op);
+  d.Int("page_size", &p.page_size);
+  if (!d.ok()) return d.Error();
+  static const char* names[] = {"RESERVE", "FORK", "FREE", "COMPACT"};
+  p.op = -1;
+  for (int i = 0; i < 4; ++i)
+    if (op == names[i]) p.op = i;
+  std::string why;
+  const int64_t batch = tab->dims[0], pages = refs->dims[0];
+  const int64_t n = p.op == XLA_AMD_KV_PAGES_FORK || p.op == XLA_AMD_KV_PAGES_FREE ? (req ? req->dims[0] : 0) : 0;
+  if (p.op < 0) why = "Unknown op `" + op + "` (RESERVE, FORK, FREE or COMPACT)";
+  else if (lens->dims[0] != batch) why = "kv_lens must have one entry per row of page_table";
+  else if (!SameShape(tab, tab_o) || !SameShape(lens, lens_o) || !SameShape(refs, refs_o))
+    why = "the new page_table, kv_lens and ref_counts must have the old ones' shapes";
+  else if ((req == nullptr) != (p.op == XLA_AMD_KV_PAGES_COMPACT)) why = "a request goes with RESERVE, FORK and FREE, and only with them";
+  else if (p.op == XLA_AMD_KV_PAGES_RESERVE && (req->rank != 1 || req->dims[0] != batch)) why = "the request of RESERVE must be [batch]";
+  else if (p.op == XLA_AMD_KV_PAGES_FORK && (req->rank != 2 || req->dims[1] != 2)) why = "the request of FORK must be [n,2]";
+  else if (p.op == XLA_AMD_KV_PAGES_FREE && req->rank != 1) why = "the request of FREE must be [n]";
+  else if (moves->dims[1] != 2 || moves->dims[0] != (p.op == XLA_AMD_KV_PAGES_FORK ? n : p.op == XLA_AMD_KV_PAGES_COMPACT ? pages / 2 : 0))
+    why = "moves must be [n,2] for FORK, [pages/2,2] for COMPACT, else [0,2]";
+  else if (status->dims[0] != (p.op == XLA_AMD_KV_PAGES_RESERVE ? batch : n))
+    why = "status must have one entry per request";
+  if (!why.empty()) return InvalidArgument(f->api, "xla_amd.kv_cache_pages: " + why);
+  p.page_table = (const int32_t*)tab->data;
+  p.kv_lens = (const int32_t*)lens->data;
+  p.ref_counts = (const int32_t*)refs->data;
+  p.request = req ? (const int32_t*)req->data : nullptr;
+  p.page_table_out = (int32_t*)tab_o->data;
+  p.kv_lens_out = (int32_t*)lens_o->data;
+  p.ref_counts_out = (int32_t*)refs_o->data;
+  p.moves = (int32_t*)moves->data;
+  p.status = (int32_t*)status->data;
+  p.workspace = ws->data;
+  p.workspace_bytes = (size_t)Elements(ws);
+  p.batch = batch;
+  p.table_width = tab->dims[1];
+  p.pages = pages;
+  p.requests = n;
+  void* stream;
+  if (XLA_FFI_Error* e = GetStream(f, &stream)) return e;
+  return LaunchStatus(f, xla_amd_launch_kv_cache_pages(&p, stream));
+}
+
+XLA_FFI_Error* xla_amd_kv_cache_copy_pages(XLA_FFI_CallFrame* f) {
+  XLA_FFI_Error* err;
+  constexpr int kMax = XLA_AMD_KV_CACHE_MAX_BUFFERS;
+  if (Preamble(f, 2, kMax + 1, 1, kMax, &err)) return err;
+  Decoder d{f};
+  XLA_FFI_Buffer* moves = d.Arg(0, Bit(XLA_FFI_DataType_S32), 2, 2, "moves");
+  const int n = (int)f->args.size - 1;
+  XLA_FFI_Buffer *in[kMax], *out[kMax];
+  for (int i = 0; i < n; ++i) in[i] = d.Arg(1 + i, kWholeByteMask, 1, 16, "buffer");
+  for (int64_t i = 0; i < f->rets.size; ++i) out[i] = d.Ret((int)i, kWholeByteMask, 1, 16, "buffer");
+  if (!d.ok()) return d.Error();
+  void* buffers[kMax];
+  int64_t page_bytes[kMax];
+  std::string why;
+  if (moves->dims[1] != 2) why = "moves must be [m,2]";
+  else if (f->rets.size != n) why = "there must be one result per buffer";
+  for (int i = 0; i < n && why.empty(); ++i) {
+    if (in[i]->dims[0] != in[0]->dims[0]) why = "all buffers must have the same number of pages";
+    else if (!SameShape(in[i], out[i]) || in[i]->dtype != out[i]->dtype || in[i]->data != out[i]->data)
+      why = "the results are the operands' own buffers (output_to_operand_aliasing)";
+    buffers[i] = in[i]->data;
+    page_bytes[i] = ElementBytes(in[i]->dtype);
+    for (int64_t r = 1; r < in[i]->rank; ++r) page_bytes[i] *= in[i]->dims[r];
+  }
+  if (!why.empty()) return InvalidArgument(f->api, "xla_amd.kv_cache_copy_pages: " + why);
+  XlaAmdKvCacheCopyPages p{};
+  p.moves = (const int32_t*)moves->data;
+  p.buffers = buffers;
+  p.page_bytes = page_bytes;
+  p.num_moves = moves->dims[0];
+  p.pages = in[0]->dims[0];
+  p.num_buffers = n;
+  void* stream;
+  if (XLA_FFI_Error* e = GetStream(f, &stream)) return e;
+  return LaunchStatus(f, xla_amd_launch_kv_cache_copy_pages(&p, stream));
+}
+
 XLA_FFI_Error* xla_amd_register_handlers(const XLA_FFI_Api* api) {
   struct Entry { const char* name; XLA_FFI_Handler* fn; };
   const Entry entries[] = {{XLA_AMD_TARGET_DEQUANT_DOT, xla_amd_dequant_dot},
                            {XLA_AMD_TARGET_FP8_SCALED_DOT, xla_amd_fp8_scaled_dot},
-                           {XLA_AMD_TARGET_QUANTIZE_FP8, xla_amd_rowwise_quantize_fp8}};
+                           {XLA_AMD_TARGET_QUANTIZE_FP8, xla_amd_rowwise_quantize_fp8},
+                           {XLA_AMD_TARGET_KV_CACHE_WRITE, xla_amd_kv_cache_write},
+                           {XLA_AMD_TARGET_KV_CACHE_ATTENTION, xla_amd_kv_cache_attention},
+                           {XLA_AMD_TARGET_KV_CACHE_PAGES, xla_amd_kv_cache_pages},
+                           {XLA_AMD_TARGET_KV_CACHE_COPY_PAGES, xla_amd_kv_cache_copy_pages}};
   for (const Entry& e : entries) {
     XLA_FFI_Handler_Register_Args args;
     memset(&args, 0, sizeof(args));

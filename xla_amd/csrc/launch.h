@@ -37,6 +37,15 @@ int LaunchFp8DotDecode(const XlaAmdFp8ScaledDot& p, hipStream_t stream, bool bf1
                        bool* any_scale = nullptr);
 size_t Fp8DotDecodeWorkspaceBytes(int64_t batch, int64_t M, int64_t K, int64_t N, int rhs_contracting_dim);
 
+// The 8-bit paged key/value cache (kv_cache_write.hip, kv_cache_attention.hip, kv_cache_pages.hip).
+int LaunchKvCacheWrite(const XlaAmdKvCacheWrite& p, hipStream_t stream);
+int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream);
+size_t KvCacheAttentionWorkspaceBytes(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_size,
+                                      int64_t max_positions);
+int LaunchKvCachePages(const XlaAmdKvCachePages& p, hipStream_t stream);
+size_t KvCachePagesWorkspaceBytes(int64_t batch, int64_t pages, int64_t requests);
+int LaunchKvCacheCopyPages(const XlaAmdKvCacheCopyPages& p, hipStream_t stream);
+
 inline bool IsF32OrBf16(int32_t t) {
   return t == XLA_FFI_DataType_F32 || t == XLA_FFI_DataType_BF16;
 }

@@ -19,13 +19,19 @@ HANDLER_SYMBOLS = {
     "xla_amd.dequant_dot": "xla_amd_dequant_dot",
     "xla_amd.fp8_scaled_dot": "xla_amd_fp8_scaled_dot",
     "xla_amd.rowwise_quantize_fp8": "xla_amd_rowwise_quantize_fp8",
+    "xla_amd.kv_cache_write": "xla_amd_kv_cache_write",
+    "xla_amd.kv_cache_attention": "xla_amd_kv_cache_attention",
+    "xla_amd.kv_cache_pages": "xla_amd_kv_cache_pages",
+    "xla_amd.kv_cache_copy_pages": "xla_amd_kv_cache_copy_pages",
 }
 EXPORTED_SYMBOLS = list(HANDLER_SYMBOLS.values()) + [
     "xla_amd_register_handlers", "xla_amd_launch_dequant_dot", "xla_amd_launch_dequant_dot_static_scratch",
     "xla_amd_launch_fp8_scaled_dot",
     "xla_amd_launch_rowwise_quantize_fp8", "xla_amd_dequant_dot_workspace_bytes", "xla_amd_dequant_dot_workspace_bytes_nk",
     "xla_amd_fp8_scaled_dot_workspace_bytes", "xla_amd_fp8_scaled_dot_workspace_bytes_typed", "xla_amd_last_error",
-    "xla_amd_last_kernel",
+    "xla_amd_last_kernel", "xla_amd_launch_kv_cache_write", "xla_amd_launch_kv_cache_attention",
+    "xla_amd_launch_kv_cache_pages", "xla_amd_launch_kv_cache_copy_pages",
+    "xla_amd_kv_cache_attention_workspace_bytes", "xla_amd_kv_cache_pages_workspace_bytes",
     "xla_amd_debug_set_option"]
 SELFCHECK_SYMBOLS = ["xla_amd_selfcheck_tanh_division_mismatches", "xla_amd_selfcheck_stream",
                      "xla_amd_selfcheck_launch_empty"]
@@ -281,6 +287,10 @@ def library():
         L.xla_amd_fp8_scaled_dot_workspace_bytes.argtypes = [C.c_int64] * 3 + [C.c_int32]
         L.xla_amd_fp8_scaled_dot_workspace_bytes_typed.restype = C.c_size_t
         L.xla_amd_fp8_scaled_dot_workspace_bytes_typed.argtypes = [C.c_int64] * 3 + [C.c_int32] * 2
+        L.xla_amd_kv_cache_attention_workspace_bytes.restype = C.c_size_t
+        L.xla_amd_kv_cache_attention_workspace_bytes.argtypes = [C.c_int64] * 6
+        L.xla_amd_kv_cache_pages_workspace_bytes.restype = C.c_size_t
+        L.xla_amd_kv_cache_pages_workspace_bytes.argtypes = [C.c_int64] * 3
         _lib = L
     return _lib
 

@@ -119,7 +119,11 @@ class Executable:
         if ins["attrs"].get("api_version") != "API_VERSION_TYPED_FFI":
             raise ValueError("custom call %s does not use the typed FFI" % ins["name"])
         res_shapes = ins["shape"]["tuple"] if "tuple" in ins["shape"] else [ins["shape"]]
-        results = [torch.empty(s["dims"], dtype=_TORCH[s["dtype"]], device="cuda") for s in res_shapes]
+        # a result that the instruction aliases with an operand is that operand's buffer
+        alias = {int(m.group(1) or 0): int(m.group(2)) for m in
+                 re.finditer(r"\{(\d*)\}:\s*\((\d+),", ins["attrs"].get("output_to_operand_aliasing", ""))}
+        results = [operands[alias[i]] if i in alias else torch.empty(s["dims"], dtype=_TORCH[s["dtype"]], device="cuda")
+                   for i, s in enumerate(res_shapes)]
         args = [(_DT[s["dtype"]], t.data_ptr(), s["dims"]) for t, s in zip(operands, operand_shapes)]
         rets = [(_DT[s["dtype"]], t.data_ptr(), s["dims"]) for t, s in zip(results, res_shapes)]
         attrs = parse_backend_config(ins["attrs"].get("backend_config", '"{}"'))

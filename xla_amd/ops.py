@@ -1,4 +1,4 @@
-"""The three custom calls as Python callables over device tensors.
+"""The custom calls as Python callables over device tensors.
 
 Every function builds an XLA FFI call frame and goes through the library's exported
 handler symbol -- the same entry XLA's CustomCallThunk would call -- on torch's current
@@ -185,4 +185,151 @@ def rowwise_quantize_fp8(x, gamma=None, *, eps=1e-6, q=None, scales=None, build_
     attrs = {"rmsnorm": ffi.Attr.pred(gamma is not None), "eps": ffi.Attr.f32(eps)}
     call = Call("xla_amd.rowwise_quantize_fp8", ffi.Frame(host(), args, rets, attrs), (q, scales),
                 keep=(x, gamma))
+    return call if build_only else call.run()
+
+
+# ---- the 8-bit paged key/value cache ---------------------------------------------------------------
+
+_CACHE = {torch.int8: dtypes.S8, torch.float8_e4m3fn: dtypes.F8E4M3FN, torch.uint8: dtypes.F8E4M3FN}
+_ANY = {torch.int8: dtypes.S8, torch.uint8: dtypes.U8, torch.float8_e4m3fn: dtypes.F8E4M3FN, torch.bool: dtypes.PRED,
+        torch.float8_e5m2: dtypes.F8E5M2, torch.bfloat16: dtypes.BF16, torch.float16: dtypes.F16, torch.int16: dtypes.S16,
+        torch.float32: dtypes.F32, torch.int32: dtypes.S32}
+
+
+def _operand(t, name, kinds, rank=None):
+    """(element type, pointer, dimensions) of a tensor that a call frame can describe: on the GPU, row-major."""
+    if t.dtype not in kinds:
+        raise TypeError("%s: element type %s is not one of %s" % (name, t.dtype, ", ".join(str(k) for k in kinds)))
+    if not t.is_contiguous():
+        raise ValueError("%s must be contiguous: a call frame has no strides" % name)
+    if rank is not None and t.dim() != rank:
+        raise ValueError("%s must have %d dimensions, got %d" % (name, rank, t.dim()))
+    return kinds[t.dtype], t.data_ptr(), list(t.shape)
+
+
+def _one_device(*tensors):
+    _check_cuda(*tensors)
+    at = {t.device for t in tensors if t is not None}
+    if len(at) > 1:
+        raise ValueError("operands lie on different devices: " + ", ".join(sorted(str(d) for d in at)))
+    return at.pop()
+
+
+class _DeviceCall(Call):
+    """A Call that runs on its operands' own device, on torch's current stream there."""
+
+    def __init__(self, device, *args, **kw):
+        super().__init__(*args, **kw)
+        self._device = device
+
+    def run(self):
+        with torch.cuda.device(self._device):
+            return super().run()
+
+
+def _cache_operands(k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets):
+    f32, s32 = {torch.float32: dtypes.F32}, {torch.int32: dtypes.S32}
+    return [_operand(k_cache, "k_cache", _CACHE, 4), _operand(v_cache, "v_cache", _CACHE, 4),
+            _operand(k_scales, "k_scales", f32, 3), _operand(v_scales, "v_scales", f32, 3),
+            _operand(page_table, "page_table", s32, 2), _operand(kv_lens, "kv_lens", s32, 1),
+            _operand(q_offsets, "q_offsets", s32, 1)]
+
+
+def kv_cache_write(k, v, k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets, *, build_only=False):
+    """Quantises the new rows k, v (bf16 [rows, kv_heads, head]) into the pages of an 8-bit cache, in place, and
+    returns (k_cache, v_cache, k_scales, v_scales).
+
+    k_cache, v_cache: codes [pages, kv_heads, page, head], int8 (s8) or float8_e4m3fn / uint8 (f8e4m3fn);
+    k_scales, v_scales: float32 [pages, kv_heads, page / block], a cached value is code * scale;
+    page_table int32 [batch, width]: position t of sequence b lies in page page_table[b, t // page];
+    kv_lens int32 [batch]: lengths with the new rows; q_offsets int32 [batch + 1]: sequence b owns rows
+    q_offsets[b] to q_offsets[b + 1], its last ones.  A block's scale is max|x| / 127 (s8) or / 448 (f8); one that
+    held rows before keeps the larger of its old and new scale and its old codes follow it."""
+    cache = (k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets)
+    device = _one_device(k, v, *cache)
+    bf16 = {torch.bfloat16: dtypes.BF16}
+    ops_ = _cache_operands(*cache)
+    args = [_operand(k, "k", bf16, 3), _operand(v, "v", bf16, 3)] + ops_
+    call = _DeviceCall(device, "xla_amd.kv_cache_write", ffi.Frame(host(), args, ops_[:4], {}),
+                       (k_cache, v_cache, k_scales, v_scales), keep=(k, v) + cache)
+    return call if build_only else call.run()
+
+
+def kv_cache_attention(q, k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets, *, scale=None,
+                       causal=True, window=0, softcap=0.0, lse=False, out=None, scratch="auto", build_only=False):
+    """Softmax attention of q (bf16 [rows, q_heads, head]) over the pages of an 8-bit cache laid out as for
+    kv_cache_write; returns out (bf16, like q), or (out, lse) with lse=True (float32 [rows, q_heads]).
+
+    q_heads is a multiple of kv_heads.  Row i of a sequence's n rows stands at position kv_lens[b] - n + i; it
+    sees the positions below kv_lens[b], up to its own if causal, and the last `window` of those if window > 0.
+    scale: softmax scale (default head ** -0.5); softcap c > 0: scores become c * tanh(score / c).
+    Rows that see nothing, or belong to no sequence, are 0 and their lse -inf."""
+    cache = (k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets)
+    device = _one_device(q, out, *cache)
+    bf16 = {torch.bfloat16: dtypes.BF16}
+    args = [_operand(q, "q", bf16, 3)] + _cache_operands(*cache)
+    if out is None:
+        out = torch.empty_like(q)
+    rets = [_operand(out, "out", bf16, 3)]
+    lse_t = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if lse else None
+    if lse:
+        rets.append(_operand(lse_t, "lse", {torch.float32: dtypes.F32}))
+    if scratch == "auto":
+        scratch = _scratch(ffi.library().xla_amd_kv_cache_attention_workspace_bytes(
+            q.shape[0], kv_lens.shape[0], q.shape[1], k_cache.shape[1], q.shape[2],
+            page_table.shape[1] * k_cache.shape[2]), device)
+    if scratch is not None:
+        rets.append((dtypes.U8, scratch.data_ptr(), [scratch.numel()]))
+    attrs = {"causal": ffi.Attr.pred(causal), "window": ffi.Attr.i64(window), "softcap": ffi.Attr.f32(softcap)}
+    if scale is not None:
+        attrs["softmax_scale"] = ffi.Attr.f32(scale)
+    call = _DeviceCall(device, "xla_amd.kv_cache_attention", ffi.Frame(host(), args, rets, attrs),
+                       (out, lse_t) if lse else out, keep=(q, out, lse_t, scratch) + cache)
+    return call if build_only else call.run()
+
+
+def kv_cache_pages(op, page_table, kv_lens, ref_counts, request=None, *, page_size, build_only=False):
+    """Book-keeping of a page pool without a step on the host: returns a new (page_table, kv_lens, ref_counts,
+    moves, status), all int32, from page_table [batch, width], kv_lens [batch] and ref_counts [pages] (0: free).
+
+    op "RESERVE": request [batch] of wanted lengths; pages are given lowest free first, in the order of the
+    sequences, until one does not fit; status [batch] is 1 where the length was granted.
+    op "FORK": request [n, 2] of (source, empty destination); full pages are shared, a last page that is not full is
+    replaced by a free one, and moves [n, 2] lists (old, new) for kv_cache_copy_pages, then -1; status [n].
+    op "FREE": request [n] of sequences; status [n] is 0 for one outside the batch or named before.
+    op "COMPACT": the pages in use move to the front; moves [pages // 2, 2], then -1.
+    moves is [0, 2] for RESERVE and FREE, status [0] for COMPACT."""
+    if op not in ("RESERVE", "FORK", "FREE", "COMPACT"):
+        raise ValueError("op must be RESERVE, FORK, FREE or COMPACT, got %r" % (op,))
+    device = _one_device(page_table, kv_lens, ref_counts, request)
+    s32 = {torch.int32: dtypes.S32}
+    args = [_operand(page_table, "page_table", s32, 2), _operand(kv_lens, "kv_lens", s32, 1),
+            _operand(ref_counts, "ref_counts", s32, 1)]
+    n = 0
+    if request is not None:
+        args.append(_operand(request, "request", s32))
+        n = request.shape[0] if request.dim() > 0 else 0
+    pages = ref_counts.shape[0]
+    new = [torch.empty_like(t) for t in (page_table, kv_lens, ref_counts)]
+    moves = torch.empty((n if op == "FORK" else pages // 2 if op == "COMPACT" else 0, 2), dtype=torch.int32, device=device)
+    status = torch.empty((n,), dtype=torch.int32, device=device)
+    scratch = _scratch(ffi.library().xla_amd_kv_cache_pages_workspace_bytes(kv_lens.shape[0], pages, n), device)
+    result = tuple(new) + (moves, status)
+    rets = [_operand(t, "result", s32) for t in result] + [(dtypes.U8, scratch.data_ptr(), [scratch.numel()])]
+    attrs = {"op": ffi.Attr.str(op), "page_size": ffi.Attr.i64(page_size)}
+    call = _DeviceCall(device, "xla_amd.kv_cache_pages", ffi.Frame(host(), args, rets, attrs), result,
+                       keep=(page_table, kv_lens, ref_counts, request, scratch))
+    return call if build_only else call.run()
+
+
+def kv_cache_copy_pages(moves, buffers, *, build_only=False):
+    """buffer[destination] = buffer[source] for every (source, destination) of moves (int32 [m, 2]) in every one of
+    `buffers` ([pages, ...], up to 64), in place; returns the buffers.  Pairs that name a page outside the pool
+    (as the -1 behind the moves of kv_cache_pages) are skipped; no destination may occur twice or be a source."""
+    buffers = list(buffers)
+    device = _one_device(moves, *buffers)
+    rets = [_operand(t, "buffer %d" % i, _ANY) for i, t in enumerate(buffers)]
+    args = [_operand(moves, "moves", {torch.int32: dtypes.S32}, 2)] + rets
+    call = _DeviceCall(device, "xla_amd.kv_cache_copy_pages", ffi.Frame(host(), args, rets, {}), buffers,
+                       keep=(moves,) + tuple(buffers))
     return call if build_only else call.run()
