@@ -6,6 +6,7 @@
 // over the positions j that the row sees, with the running maximum m and sum of a softmax.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <stdio.h>
 
 #include "kv_cache.h"
 
@@ -22,93 +23,595 @@ struct AttentionView {
   int causal, window;
 };
 
-template <bool F8>
-__device__ __forceinline__ float code_value(uint32_t c) {
-  if constexpr (F8) return f8e4m3fn_to_f32(c);
-  return (float)(int8_t)c;
+// ---- few rows for each sequence: the cache is streamed once ------------------------------------------
+//
+// A workgroup of four waves takes the packed rows (row, head of the group) of one sequence and cache head, 16
+// or 32 at a time, along a range of 128-position units, 32 positions a wave; each wave has its own running
+// maximum, sum and result, which meet in LDS at the end of the range.  Per wave and 32 positions, with c = lane & 15 and
+// g = lane >> 4:
+//   S^T = K Q^T   a lane holds 16-byte pieces of key rows c straight from memory, widened to bf16 (exact for
+//                 both code types); the result has column (row of q) c and keys 4 g + i of either 16.
+//   O^T = V^T P^T the scores of a lane are, without moving, the operand's keys 4 g + i of both 16s; a lane holds
+//                 values d = c DP/16 .. of those eight keys, transposed in registers while they are widened.
+// The sums over d and over keys run in whatever order the operands share, so nothing is shuffled but maxima.
+// Scales stay out of the operands: the key's on the f32 score, the value's on the weight, which is rounded to
+// bf16 there (2^-9 of each weight, where the result is rounded by as much; f32 sums).
+//
+// Where the keys are split: all sequences' units (times their tiles of rows) stand in one line, which is cut
+// into as many equal pieces as there are workers for a head, so a batch of mixed lengths fills the device
+// evenly.  A range that covers a tile whole writes the result; any other writes f32 sums to the
+// scratch, at most two for each worker, and a second launch joins them in order.
+//
+// Bound: HBM, 2 (head + 4 / block) bytes for each position and cache head.
+constexpr int kUnit = 128;
+
+struct DecodeView {
+  AttentionView a;
+  float* partial;   // [heads][2 * workers][tile rows][head + 2], or null: ranges are whole tiles
+  int workers;      // for each head
+  int rows_from, rows_to;  // sequences with rows_from < n * group <= rows_to are this kernel's
+};
+
+// Tiles of packed rows of a sequence and the units of positions that any of its rows sees.
+struct DecodeSpan {
+  KvSequence s;
+  int lo, hi;  // positions [lo, hi)
+  int tiles, units, first;  // first: the first unit
+};
+
+template <int RT>
+__device__ __forceinline__ DecodeSpan decode_span(const DecodeView& v, int b) {
+  DecodeSpan r;
+  r.s = kv_sequence(v.a.c, b);
+  const int rows = r.s.n * v.a.group;
+  r.lo = v.a.window > 0 ? max(0, r.s.len - r.s.n - v.a.window + 1) : 0;
+  r.hi = r.s.len;
+  const bool mine = rows > v.rows_from && rows <= v.rows_to;
+  r.tiles = mine ? (rows + RT - 1) / RT : 0;
+  r.first = r.lo / kUnit;
+  r.units = max((r.hi + kUnit - 1) / kUnit - r.first, 1);  // a sequence that sees nothing has its zeros written
+  return r;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = __builtin_fmaxf(v, __shfl_xor(v, off));
-  return v;
-}
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
-  return v;
+__device__ __forceinline__ int64_t shfl64(int64_t x, int src) {
+  const int lo = __shfl((int)(uint32_t)(uint64_t)x, src), hi = __shfl((int)(uint32_t)((uint64_t)x >> 32), src);
+  return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
 }
 
-// One wave for a row and head: 64 positions at a time, a lane each for the scores, then the lanes go along
-// the head for the values.
-template <bool F8>
-__global__ __launch_bounds__(64) void kv_cache_attention_row_kernel(AttentionView v) {
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uint64_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// The units of all sequences together.
+template <int RT>
+__device__ int64_t decode_total(const DecodeView& v, int lane) {
+  int64_t sum = 0;
+  for (int b = lane; b < v.a.c.batch; b += 64) {
+    const DecodeSpan s = decode_span<RT>(v, b);
+    sum += (int64_t)s.tiles * s.units;
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += shfl64(sum, lane ^ off);
+  return sum;
+}
+
+// The sequence that holds entry `at` of the line, where entries are its units (TILES false) or tiles, and how
+// many entries and units lie before it; -1 past the end.
+template <int RT, bool TILES>
+__device__ int decode_find(const DecodeView& v, int64_t at, int lane, int64_t* before, int64_t* units_before) {
+  int64_t seen = 0, seen_units = 0;
+  for (int b0 = 0; b0 < v.a.c.batch; b0 += 64) {
+    int64_t n = 0, u = 0;
+    if (b0 + lane < v.a.c.batch) {
+      const DecodeSpan s = decode_span<RT>(v, b0 + lane);
+      u = (int64_t)s.tiles * s.units;
+      n = TILES ? s.tiles : u;
+    }
+    int64_t incl = n, incl_u = u;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t t = shfl64(incl, lane - off);
+      if (lane >= off) incl += t;
+      if (TILES) {
+        const int64_t tu = shfl64(incl_u, lane - off);
+        if (lane >= off) incl_u += tu;
+      }
+    }
+    if (!TILES) incl_u = incl;
+    const unsigned long long hit = __ballot(at < seen + incl && n > 0 && at >= seen + incl - n);
+    if (hit != 0ull) {
+      const int src = __builtin_ctzll(hit);
+      *before = seen + shfl64(incl - n, src);
+      *units_before = seen_units + shfl64(incl_u - u, src);
+      return __builtin_amdgcn_readfirstlane(b0 + src);
+    }
+    seen += shfl64(incl, 63);
+    seen_units += shfl64(incl_u, 63);
+  }
+  return -1;
+}
+
+// First unit of worker w when `total` units are cut into `workers` pieces.
+__device__ __forceinline__ int64_t worker_start(int64_t total, int workers, int w) { return total * w / workers; }
+__device__ __forceinline__ int workers_used(int64_t total, int workers) { return (int)min((int64_t)workers, total); }
+
+// Two codes at byte places i, i + 1 -> two bf16 in a dword, exact.
+template <bool F8, int I>
+__device__ __forceinline__ uint32_t widen2(uint32_t w) {
+  if constexpr (F8) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, I != 0));
+  } else {
+    const float a = (float)(int8_t)(w >> (8 * I)), b = (float)(int8_t)(w >> (8 * I + 8));
+    return __builtin_amdgcn_perm(f32_to_bits(b), f32_to_bits(a), 0x07060302u);
+  }
+}
+
+// Byte t of eight keys (word W = t / 4 of each) -> eight bf16.
+template <bool F8, int T, int N>
+__device__ __forceinline__ bf16x8 column8(const uint32_t (&k)[8][N]) {
+  constexpr int W = T >> 2, I = T & 3;
+  uintx4 r;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) {
+    const uint32_t a = k[2 * p][W], b = k[2 * p + 1][W];
+    if constexpr (F8) {
+      // bytes I of both keys in the low half, where the conversion reads them
+      const uint32_t pair = __builtin_amdgcn_perm(b, a, 0x0c0c0000u | ((4 + I) << 8) | I);
+      r[p] = widen2<true, 0>(pair);
+    } else {
+      const float x = (float)(int8_t)(a >> (8 * I)), y = (float)(int8_t)(b >> (8 * I));
+      r[p] = __builtin_amdgcn_perm(f32_to_bits(y), f32_to_bits(x), 0x07060302u);
+    }
+  }
+  return __builtin_bit_cast(bf16x8, r);
+}
+
+// Rows first to first + 63, where they belong to no sequence: 0, lse -infinity.
+__device__ void clear_rows_of_nobody(const AttentionView& v, int first) {
   const KvCacheView& c = v.c;
-  const int lane = threadIdx.x, row = blockIdx.x, qh = blockIdx.y, head = qh / v.group;
-  __shared__ float q[256], weight[64];
-  __shared__ int page_of[64];
-  const int64_t at = ((int64_t)row * v.q_heads + qh) * c.head;
-  for (int d = lane; d < c.head; d += 64) q[d] = bf16_to_f32(v.q[at + d]);
-  int b = -1;
-  for (int b0 = 0; b0 < c.batch && b < 0; b0 += 64) {
-    bool mine = false;
-    if (b0 + lane < c.batch) {
-      const KvSequence s = kv_sequence(c, b0 + lane);
-      mine = row >= s.row0 && row < s.row0 + s.n;
-    }
-    const unsigned long long hit = __ballot(mine);
-    if (hit != 0ull) b = b0 + __builtin_ctzll(hit);
-  }
-  float m = -INFINITY, sum = 0.0f, acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (b >= 0) {
+  __shared__ int owned[64];
+  if (threadIdx.x < 64) owned[threadIdx.x] = 0;
+  __syncthreads();
+  for (int b = threadIdx.x; b < c.batch; b += blockDim.x) {
     const KvSequence s = kv_sequence(c, b);
-    const int pos = s.len - s.n + (row - s.row0);
-    const int end = v.causal ? min(s.len, pos + 1) : s.len;
-    const int begin = v.window > 0 ? max(0, pos - v.window + 1) : 0;
-    const int in_page = (1 << c.page_log2) - 1;
-    for (int j0 = begin; j0 < end; j0 += 64) {
-      const int j = j0 + lane;
-      const int page = j < end ? kv_page(c, b, j) : -1;
-      float x = -INFINITY, vs = 0.0f;
-      if (page >= 0) {
-        const uint8_t* k = c.codes[0] + kv_row(c, page, head, j & in_page);
-        float dot = 0.0f;
-        for (int d = 0; d < c.head; ++d) dot = __builtin_fmaf(q[d], code_value<F8>(k[d]), dot);
-        x = dot * (c.scales[0][kv_scale(c, page, head, j & in_page)] * v.scale);
-        if (v.softcap > 0.0f) x = v.softcap * tanhf(x / v.softcap);
-        vs = c.scales[1][kv_scale(c, page, head, j & in_page)];
+    const int from = max(s.row0, first), to = min(s.row0 + s.n, first + 64);
+    for (int r = from; r < to; ++r) owned[r - first] = 1;
+  }
+  __syncthreads();
+  for (int r = 0; r < 64 && first + r < c.rows; ++r) {
+    if (owned[r]) continue;
+    const int64_t at = (int64_t)(first + r) * v.q_heads;
+    uintx4* o = reinterpret_cast<uintx4*>(v.out + at * c.head);
+    for (int i = threadIdx.x; i < v.q_heads * c.head / 8; i += blockDim.x) o[i] = uintx4{0u, 0u, 0u, 0u};
+    if (v.lse)
+      for (int i = threadIdx.x; i < v.q_heads; i += blockDim.x) v.lse[at + i] = -INFINITY;
+  }
+}
+
+// What a wave has under way for 32 positions: key and value codes of both 16s, and their scales.
+template <int DP, bool SMALL>
+struct DecodeLoads {
+  static constexpr int S = SMALL ? 4 : 1;
+  uintx4 k[2][DP / 64];
+  uint32_t v[8][DP / 64];
+  float ks[2][S], vs[2][S];
+  bool there[2];
+};
+
+template <bool F8, int DP, int QT, bool SMALL>
+__global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeView v) {
+  constexpr int RT = 16 * QT;        // packed rows of a tile
+  constexpr int KW = DP / 64;        // 16-byte pieces of a key row that a lane holds
+  constexpr int VT = DP / 16;        // values of a position that a lane holds
+  constexpr int NF = DP + 4;         // row stride of the sums in LDS
+  __shared__ float sums[4][16 * NF];
+  __shared__ float tops[4][RT], totals[4][RT];
+  const KvCacheView& c = v.a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, grp = lane >> 4;
+  const int head = blockIdx.y;
+  if ((int)blockIdx.x >= v.workers) {
+    if (head == 0) clear_rows_of_nobody(v.a, 64 * (blockIdx.x - v.workers));
+    return;
+  }
+  const int64_t total = uniform64(decode_total<RT>(v, lane));
+  const int used = v.partial ? workers_used(total, v.workers) : v.workers;
+  if (total == 0 || (int)blockIdx.x >= used) return;
+  int64_t pos = worker_start(total, used, blockIdx.x);
+  const int64_t stop = worker_start(total, used, blockIdx.x + 1);
+  int64_t before, ignored;
+  int b = decode_find<RT, false>(v, pos, lane, &before, &ignored);
+  before = uniform64(before);
+
+  // byte offsets of a lane inside 16 rows of a page and head; a head shorter than DP repeats its end, which
+  // q's zeros cancel on one side and the results beyond it are dropped on the other
+  const int stride = c.head;
+  uint32_t koff[KW], voff[4];
+#pragma unroll
+  for (int s = 0; s < KW; ++s) koff[s] = (uint32_t)(col * stride + min(grp * (DP / 4) + 16 * s, stride - 16));
+#pragma unroll
+  for (int i = 0; i < 4; ++i) voff[i] = (uint32_t)((4 * grp + i) * stride + min(col * VT, stride - VT));
+  const float to_log2 = 1.44269504088896341f;
+  const float cap = v.a.softcap;
+  // scores in units of log 2: exp2 takes them as they are
+  const float factor = cap > 0.0f ? v.a.scale : v.a.scale * to_log2;
+  const int in_page = (1 << c.page_log2) - 1;
+
+  while (b >= 0 && b < c.batch && pos < stop) {
+    const DecodeSpan sp = decode_span<RT>(v, b);
+    if (sp.tiles == 0) {
+      ++b;
+      continue;
+    }
+    const int64_t at = pos - before;  // inside the sequence
+    const int tile = (int)(at / sp.units);
+    if (tile >= sp.tiles) {
+      before += (int64_t)sp.tiles * sp.units;
+      ++b;
+      continue;
+    }
+    const int u0 = (int)(at - (int64_t)tile * sp.units);
+    int u1 = (int)min((int64_t)sp.units, (int64_t)u0 + (stop - pos));
+    if (!v.partial) {
+      // whole tiles: the worker in whose range a tile begins has all of it
+      if (u0 != 0) {
+        pos += sp.units - u0;
+        continue;
       }
-      const float top = __builtin_fmaxf(m, wave_max(x));
-      const float rescale = m == -INFINITY ? 0.0f : expf(m - top);
-      const float p = page >= 0 ? expf(x - top) : 0.0f;
-      sum = sum * rescale + wave_sum(p);
-      m = top;
-      __syncthreads();
-      weight[lane] = page >= 0 ? p * vs : 0.0f;
-      page_of[lane] = page;
-      __syncthreads();
+      u1 = sp.units;
+    }
+    pos += u1 - u0;
+
+    // the tile's rows: packed row r is row r / group and head r % group
+    const int r0 = tile * RT, rows = min(sp.s.n * v.a.group - r0, RT);
+    bf16x8 q[QT][DP / 32];
+    int sees_lo[QT], sees_hi[QT];  // positions that this lane's row sees
+    int all_lo = sp.lo, all_hi = sp.hi;  // ... and that every row of the tile sees
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] *= rescale;
-      for (int t = 0; t < min(64, end - j0); ++t) {
-        if (page_of[t] < 0) continue;
-        const uint8_t* w = c.codes[1] + kv_row(c, page_of[t], head, (j0 + t) & in_page);
+    for (int t = 0; t < QT; ++t) {
+      const int r = r0 + min(16 * t + col, rows - 1);
+      const int i = r / v.a.group, h = r - i * v.a.group;
+      const uint16_t* qr = v.a.q + ((int64_t)(sp.s.row0 + i) * v.a.q_heads + head * v.a.group + h) * c.head;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (lane + 64 * i < c.head) acc[i] = __builtin_fmaf(weight[t], code_value<F8>(w[lane + 64 * i]), acc[i]);
+      for (int s = 0; s < DP / 32; ++s) {
+        const int d = grp * (DP / 4) + 8 * s;
+        q[t][s] = d < c.head ? *reinterpret_cast<const bf16x8*>(qr + d) : bf16x8{};
+      }
+      const int p = sp.s.len - sp.s.n + i;
+      sees_hi[t] = v.a.causal ? min(sp.hi, p + 1) : sp.hi;
+      sees_lo[t] = v.a.window > 0 ? max(0, p - v.a.window + 1) : 0;
+    }
+    if (v.a.causal) all_hi = min(all_hi, sp.s.len - sp.s.n + r0 / v.a.group + 1);
+    if (v.a.window > 0) all_lo = max(0, sp.s.len - sp.s.n + (r0 + rows - 1) / v.a.group - v.a.window + 1);
+
+    floatx4 acc[QT][VT];
+    float top[QT], sum[QT];
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      top[t] = -1e30f;  // below every score, and finite
+      sum[t] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < VT; ++i) acc[t][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    const int* table = c.table + (int64_t)b * c.width;
+    auto load = [&](int j0, DecodeLoads<DP, SMALL>& x) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = j0 + 16 * h;
+        int page = -1;
+        if (j < sp.hi && j + 16 > sp.lo) page = table[j >> c.page_log2];
+        page = __builtin_amdgcn_readfirstlane(page);
+        x.there[h] = (unsigned)page < (unsigned)c.pages;
+        if (x.there[h]) {
+          const int row = j & in_page;
+          const int64_t at = kv_row(c, page, head, row);
+          const uint8_t* kp = c.codes[0] + at;
+          const uint8_t* vp = c.codes[1] + at;
+#pragma unroll
+          for (int s = 0; s < KW; ++s) x.k[h][s] = *reinterpret_cast<const uintx4*>(kp + koff[s]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint8_t* p = vp + voff[i];
+            if constexpr (DP == 64) {
+              x.v[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(p);
+            } else if constexpr (DP == 128) {
+              const uintx2 w = *reinterpret_cast<const uintx2*>(p);
+              x.v[4 * h + i][0] = w[0];
+              x.v[4 * h + i][1] = w[1];
+            } else {
+              const uintx4 w = *reinterpret_cast<const uintx4*>(p);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x.v[4 * h + i][e] = w[e];
+            }
+          }
+          const int64_t sc = kv_scale(c, page, head, 0);
+#pragma unroll
+          for (int i = 0; i < DecodeLoads<DP, SMALL>::S; ++i) {
+            const int o = (row + 4 * grp + i) >> c.block_log2;
+            x.ks[h][i] = c.scales[0][sc + o];
+            x.vs[h][i] = c.scales[1][sc + o];
+          }
+        } else {
+#pragma unroll
+          for (int s = 0; s < KW; ++s) x.k[h][s] = uintx4{0u, 0u, 0u, 0u};
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int e = 0; e < KW; ++e) x.v[4 * h + i][e] = 0u;
+#pragma unroll
+          for (int i = 0; i < DecodeLoads<DP, SMALL>::S; ++i) x.ks[h][i] = x.vs[h][i] = 0.0f;
+        }
+      }
+    };
+    auto step = [&](int j0, DecodeLoads<DP, SMALL>& x) {
+      if (!x.there[0] && !x.there[1]) return;
+      const bool edge = j0 < all_lo || j0 + 32 > all_hi || !x.there[0] || !x.there[1];
+      if (F8 && (j0 < sp.lo || j0 + 32 > sp.hi)) {
+        // positions that nobody sees may hold NaN codes, which a weight of zero does not cancel
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = j0 + 16 * (e >> 2) + 4 * grp + (e & 3);
+          const bool keep = j >= sp.lo && j < sp.hi;
+#pragma unroll
+          for (int w = 0; w < KW; ++w) x.v[e][w] = keep ? x.v[e][w] : 0u;
+        }
+      }
+      floatx4 s[QT][2];
+#pragma unroll
+      for (int t = 0; t < QT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) s[t][h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int m = 0; m < DP / 32; ++m) {
+          uintx4 w;
+          const uint32_t a = x.k[h][m >> 1][2 * (m & 1)], bb = x.k[h][m >> 1][2 * (m & 1) + 1];
+          w[0] = widen2<F8, 0>(a);
+          w[1] = widen2<F8, 2>(a);
+          w[2] = widen2<F8, 0>(bb);
+          w[3] = widen2<F8, 2>(bb);
+          const bf16x8 kk = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+          for (int t = 0; t < QT; ++t) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[t][m], s[t][h], 0, 0, 0);
+        }
+      bf16x8 p[QT];
+#pragma unroll
+      for (int t = 0; t < QT; ++t) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int h = e >> 2, i = SMALL ? (e & 3) : 0;
+          y[e] = s[t][h][e & 3] * (x.ks[h][i] * factor);
+          if (cap > 0.0f) {
+            // cap * tanh(y / cap), in units of log 2
+            const float z = __builtin_amdgcn_exp2f(y[e] * (2.0f * to_log2 / cap));
+            y[e] = (cap * to_log2) * (1.0f - 2.0f / (1.0f + z));
+          }
+        }
+        if (edge) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int j = j0 + 16 * (e >> 2) + 4 * grp + (e & 3);
+            y[e] = x.there[e >> 2] && j >= sees_lo[t] && j < sees_hi[t] ? y[e] : -INFINITY;
+          }
+        }
+        float most = y[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) most = __builtin_fmaxf(most, y[e]);
+        // the maximum in use may lag behind by up to 2^8, which f32 and bf16 weights bear
+        if (__any(most > top[t] + 8.0f)) {
+          most = __builtin_fmaxf(most, __shfl_xor(most, 16));
+          most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+          const float now = __builtin_fmaxf(top[t], most);
+          const float scale = __builtin_amdgcn_exp2f(top[t] - now);
+          top[t] = now;
+          sum[t] *= scale;
+#pragma unroll
+          for (int i = 0; i < VT; ++i) acc[t][i] *= scale;
+        }
+        uintx4 w;
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const int h = e >> 2;
+          const float p0 = __builtin_amdgcn_exp2f(y[e] - top[t]), p1 = __builtin_amdgcn_exp2f(y[e + 1] - top[t]);
+          sum[t] += p0 + p1;
+          const float v0 = x.vs[h][SMALL ? (e & 3) : 0], v1 = x.vs[h][SMALL ? (e & 3) + 1 : 0];
+          // a weight of zero cancels no NaN or infinite scale
+          w[e >> 1] = edge ? pack_bf16x2(y[e] == -INFINITY ? 0.0f : p0 * v0, y[e + 1] == -INFINITY ? 0.0f : p1 * v1)
+                           : pack_bf16x2(p0 * v0, p1 * v1);
+        }
+        p[t] = __builtin_bit_cast(bf16x8, w);
+      }
+      static_for<0, VT>([&](auto i) {
+        const bf16x8 vv = column8<F8, decltype(i)::value>(x.v);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[t], acc[t][i], 0, 0, 0);
+      });
+    };
+
+    // two sets of loads take turns: the next 32 positions are under way while these are worked on
+    const int j_end = (sp.first + u1) * kUnit;
+    int j = (sp.first + u0) * kUnit + 32 * wave;
+    DecodeLoads<DP, SMALL> x0, x1;
+    load(j, x0);
+    while (j < j_end) {
+      load(j + kUnit < j_end ? j + kUnit : 0x7fffff00, x1);
+      step(j, x0);
+      j += kUnit;
+      if (j >= j_end) break;
+      load(j + kUnit < j_end ? j + kUnit : 0x7fffff00, x0);
+      step(j, x1);
+      j += kUnit;
+    }
+
+    // the four waves' sums, 16 rows at a time
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      sum[t] += __shfl_xor(sum[t], 16);
+      sum[t] += __shfl_xor(sum[t], 32);
+      if (grp == 0) {
+        tops[wave][16 * t + col] = top[t];
+        totals[wave][16 * t + col] = sum[t];
       }
     }
-  }
+    const bool whole = u0 == 0 && u1 == sp.units;
+    // a range that begins inside a tile is its worker's first, one that ends inside its last
+    float* part = v.partial + ((int64_t)head * 2 * v.workers + 2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * RT * (c.head + 2);
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (lane + 64 * i < c.head) v.out[at + lane + 64 * i] = f32_to_bf16(sum == 0.0f ? 0.0f : acc[i] / sum);
-  if (v.lse && lane == 0) v.lse[(int64_t)row * v.q_heads + qh] = sum == 0.0f ? -INFINITY : m + logf(sum);
+    for (int t = 0; t < QT; ++t) {
+      __syncthreads();
+      {
+        const int r = 16 * t + col;
+        const float m = __builtin_fmaxf(__builtin_fmaxf(tops[0][r], tops[1][r]), __builtin_fmaxf(tops[2][r], tops[3][r]));
+        const float scale = __builtin_amdgcn_exp2f(top[t] - m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float* o = &sums[wave][col * NF + (4 * grp + i) * VT];
+#pragma unroll
+          for (int n = 0; n < VT; n += 4)
+            *reinterpret_cast<floatx4*>(o + n) = floatx4{acc[t][n][i], acc[t][n + 1][i], acc[t][n + 2][i], acc[t][n + 3][i]} * scale;
+        }
+      }
+      __syncthreads();
+      const int r = 16 * t + (tid >> 4);
+      if (r < rows) {
+        const float m = __builtin_fmaxf(__builtin_fmaxf(tops[0][r], tops[1][r]), __builtin_fmaxf(tops[2][r], tops[3][r]));
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) l += totals[w][r] * __builtin_amdgcn_exp2f(tops[w][r] - m);
+        const int i = (r0 + r) / v.a.group, h = r0 + r - i * v.a.group;
+        const int64_t at_row = (int64_t)(sp.s.row0 + i) * v.a.q_heads + head * v.a.group + h;
+        const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+        for (int d = (tid & 15) * 4; d < c.head; d += 64) {
+          floatx4 o = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int w = 0; w < 4; ++w) o += *reinterpret_cast<const floatx4*>(&sums[w][(tid >> 4) * NF + d]);
+          if (whole) {
+            const uintx2 packed = {pack_bf16x2(o[0] * inverse, o[1] * inverse), pack_bf16x2(o[2] * inverse, o[3] * inverse)};
+            *reinterpret_cast<uintx2*>(v.a.out + at_row * c.head + d) = packed;
+          } else {
+            *reinterpret_cast<floatx4*>(part + r * c.head + d) = o;
+          }
+        }
+        if ((tid & 15) == 0) {
+          if (!whole) {
+            part[RT * c.head + r] = m;
+            part[RT * c.head + RT + r] = l;
+          } else if (v.a.lse) {
+            v.a.lse[at_row] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+          }
+        }
+      }
+    }
+    __syncthreads();  // tops and sums are the next range's
+  }
+}
+
+// Joins the sums of the workers that share a tile, in their order; one workgroup for a tile and head.
+template <int RT>
+__global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(DecodeView v) {
+  const KvCacheView& c = v.a.c;
+  const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
+  const int64_t total = decode_total<RT>(v, lane);
+  const int used = workers_used(total, v.workers);
+  int64_t tiles_before, units_before;
+  const int b = decode_find<RT, true>(v, blockIdx.x, lane, &tiles_before, &units_before);
+  if (b < 0) return;
+  const DecodeSpan sp = decode_span<RT>(v, b);
+  const int tile = (int)(blockIdx.x - tiles_before);
+  const int64_t from = units_before + (int64_t)tile * sp.units, to = from + sp.units;
+  int w0 = (int)min(from * used / total, (int64_t)used - 1);
+  while (worker_start(total, used, w0 + 1) <= from) ++w0;
+  while (worker_start(total, used, w0) > from) --w0;
+  int w1 = w0;
+  while (worker_start(total, used, w1 + 1) < to) ++w1;
+  if (w0 == w1) return;  // one worker had it all
+  const int r0 = tile * RT, rows = min(sp.s.n * v.a.group - r0, RT);
+  const int64_t size = (int64_t)RT * (c.head + 2);
+  const float* base = v.partial + (int64_t)head * 2 * v.workers * size;
+  auto part = [&](int w) { return base + (2 * w + (worker_start(total, used, w) <= from ? 1 : 0)) * size; };
+  for (int r = tid >> 4; r < rows; r += 16) {
+    float m = -1e30f;
+    for (int w = w0; w <= w1; ++w) m = __builtin_fmaxf(m, part(w)[RT * c.head + r]);
+    float l = 0.0f;
+    floatx4 o[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int w = w0; w <= w1; ++w) {
+      const float* p = part(w);
+      const float scale = __builtin_amdgcn_exp2f(p[RT * c.head + r] - m);
+      l += p[RT * c.head + RT + r] * scale;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = (tid & 15) * 4 + 64 * i;
+        if (d < c.head) o[i] += *reinterpret_cast<const floatx4*>(p + r * c.head + d) * scale;
+      }
+    }
+    const int i0 = (r0 + r) / v.a.group, h = r0 + r - i0 * v.a.group;
+    const int64_t at_row = (int64_t)(sp.s.row0 + i0) * v.a.q_heads + head * v.a.group + h;
+    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = (tid & 15) * 4 + 64 * i;
+      if (d < c.head) {
+        const uintx2 packed = {pack_bf16x2(o[i][0] * inverse, o[i][1] * inverse), pack_bf16x2(o[i][2] * inverse, o[i][3] * inverse)};
+        *reinterpret_cast<uintx2*>(v.a.out + at_row * c.head + d) = packed;
+      }
+    }
+    if ((tid & 15) == 0 && v.a.lse) v.a.lse[at_row] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+  }
+}
+
+
+// How a call runs, from its shapes alone (lengths are device data).
+struct DecodePlan {
+  int dp, qt;       // padded head; tiles of 16 rows
+  int64_t tiles;    // at most
+  int workers;      // for each cache head
+  bool split;       // whether a tile can be cut at all
+  size_t bytes;     // of scratch for the cut tiles' sums
+};
+
+DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head, int64_t positions) {
+  DecodePlan d;
+  const int64_t group = q_heads / kv_heads;
+  d.dp = head <= 64 ? 64 : head <= 128 ? 128 : 256;
+  const int64_t mean = batch > 0 ? (rows + batch - 1) / batch * group : 0;
+  d.qt = mean <= 16 ? 1 : 2;
+  d.tiles = rows * group / (16 * d.qt) + batch;
+  const int64_t units = d.tiles * ((positions + kUnit - 1) / kUnit);
+  const int64_t slots = 512;
+  int64_t w = (slots + kv_heads - 1) / kv_heads;
+  if (w > units) w = units;
+  d.workers = w < 1 ? 1 : (int)w;
+  d.split = positions > kUnit && batch > 0;
+  d.bytes = d.split ? (size_t)(kv_heads * 2 * d.workers * 16 * d.qt * (head + 2)) * 4 : 0;
+  return d;
+}
+
+template <bool F8, int DP, int QT>
+void LaunchDecode(const DecodeView& v, dim3 grid, hipStream_t stream) {
+  if (v.a.c.block_log2 < 2) kv_cache_attention_decode_kernel<F8, DP, QT, true><<<grid, 256, 0, stream>>>(v);
+  else kv_cache_attention_decode_kernel<F8, DP, QT, false><<<grid, 256, 0, stream>>>(v);
+}
+
+template <bool F8>
+void LaunchDecode(const DecodePlan& d, const DecodeView& v, dim3 grid, hipStream_t stream) {
+  if (d.dp == 64) d.qt == 1 ? LaunchDecode<F8, 64, 1>(v, grid, stream) : LaunchDecode<F8, 64, 2>(v, grid, stream);
+  else if (d.dp == 128) d.qt == 1 ? LaunchDecode<F8, 128, 1>(v, grid, stream) : LaunchDecode<F8, 128, 2>(v, grid, stream);
+  else d.qt == 1 ? LaunchDecode<F8, 256, 1>(v, grid, stream) : LaunchDecode<F8, 256, 2>(v, grid, stream);
 }
 
 }  // namespace
 
 size_t KvCacheAttentionWorkspaceBytes(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_size,
                                       int64_t max_positions) {
-  return 0;
+  if (rows <= 0 || batch <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_size <= 0 || max_positions <= 0) return 0;
+  return PlanDecode(rows, batch, q_heads, kv_heads, head_size, max_positions).bytes;
 }
 
 int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) {
@@ -122,6 +625,7 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   if (!(p.softcap >= 0.0f) || !(p.softcap < INFINITY)) return Fail(kBad, "kv_cache_attention: softcap must be a number that is not negative");
   if (!(p.softmax_scale > -INFINITY && p.softmax_scale < INFINITY))
     return Fail(kBad, "kv_cache_attention: softmax_scale must be a number");
+  if (p.cache.rows * p.q_heads > INT32_MAX) return Fail(kBad, "kv_cache_attention: at most 2^31 - 1 rows times heads");
   if (v.c.rows > 0 && (!p.q || !p.out)) return Fail(kBad, "kv_cache_attention: null q or out");
   if ((((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)p.workspace) & 15) != 0 || ((uintptr_t)p.lse & 3) != 0)
     return Fail(kBad, "kv_cache_attention: q, out and scratch must be aligned to 16 bytes, lse to 4");
@@ -134,11 +638,26 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   v.scale = p.softmax_scale;
   v.softcap = p.softcap;
   v.causal = p.causal;
-  v.window = p.window > INT32_MAX ? 0 : (int)p.window;  // no position lies further back
-  const dim3 grid((unsigned)v.c.rows, (unsigned)v.q_heads);
-  SetLastKernel("kv_cache_attention_row");
-  if (p.cache.cache_dtype == XLA_FFI_DataType_F8E4M3FN) kv_cache_attention_row_kernel<true><<<grid, 64, 0, stream>>>(v);
-  else kv_cache_attention_row_kernel<false><<<grid, 64, 0, stream>>>(v);
+  const int64_t positions = p.cache.table_width * p.cache.page_size;
+  v.window = p.window >= positions ? 0 : (int)p.window;  // every position that a causal row sees is nearer
+  const DecodePlan d = PlanDecode(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, positions);
+  DecodeView dv{};
+  dv.a = v;
+  dv.workers = d.workers;
+  dv.rows_to = INT32_MAX;
+  if (d.split && p.workspace && p.workspace_bytes >= d.bytes) dv.partial = (float*)p.workspace;
+  const dim3 grid((unsigned)(d.workers + (v.c.rows + 63) / 64), (unsigned)v.c.heads);
+  char name[64];
+  const bool f8 = p.cache.cache_dtype == XLA_FFI_DataType_F8E4M3FN;
+  snprintf(name, sizeof(name), "kv_cache_attention_decode_%s_d%d_m%d%s", f8 ? "f8" : "s8", d.dp, 16 * d.qt, dv.partial ? "_split" : "");
+  SetLastKernel(name);
+  if (f8) LaunchDecode<true>(d, dv, grid, stream);
+  else LaunchDecode<false>(d, dv, grid, stream);
+  if (dv.partial) {
+    const dim3 join((unsigned)d.tiles, (unsigned)v.c.heads);
+    if (d.qt == 1) kv_cache_attention_join_kernel<16><<<join, 256, 0, stream>>>(dv);
+    else kv_cache_attention_join_kernel<32><<<join, 256, 0, stream>>>(dv);
+  }
   return CheckLaunch("kv_cache_attention");
 }
 
