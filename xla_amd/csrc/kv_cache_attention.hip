@@ -190,6 +190,15 @@ __device__ void clear_rows_of_nobody(const AttentionView& v, int first) {
   }
 }
 
+// A value scale that is NaN or infinite moves to the score, as NaN: there it reaches the rows that see the
+// position and no others, while a weight of zero would not cancel it.
+__device__ __forceinline__ void keep_to_its_rows(float& key_scale, float& value_scale) {
+  if (!(__builtin_fabsf(value_scale) < INFINITY)) {
+    key_scale = bits_to_f32(0x7fc00000u);
+    value_scale = 0.0f;
+  }
+}
+
 // What a wave has under way for 32 positions: key and value codes of both 16s, and their scales.
 template <int DP, bool SMALL>
 struct DecodeLoads {
@@ -359,6 +368,10 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
           for (int w = 0; w < KW; ++w) x.v[e][w] = keep ? x.v[e][w] : 0u;
         }
       }
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < DecodeLoads<DP, SMALL>::S; ++i) keep_to_its_rows(x.ks[h][i], x.vs[h][i]);
       floatx4 s[QT][2];
 #pragma unroll
       for (int t = 0; t < QT; ++t)
@@ -420,9 +433,7 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
           const float p0 = __builtin_amdgcn_exp2f(y[e] - top[t]), p1 = __builtin_amdgcn_exp2f(y[e + 1] - top[t]);
           sum[t] += p0 + p1;
           const float v0 = x.vs[h][SMALL ? (e & 3) : 0], v1 = x.vs[h][SMALL ? (e & 3) + 1 : 0];
-          // a weight of zero cancels no NaN or infinite scale
-          w[e >> 1] = edge ? pack_bf16x2(y[e] == -INFINITY ? 0.0f : p0 * v0, y[e + 1] == -INFINITY ? 0.0f : p1 * v1)
-                           : pack_bf16x2(p0 * v0, p1 * v1);
+          w[e >> 1] = pack_bf16x2(p0 * v0, p1 * v1);
         }
         p[t] = __builtin_bit_cast(bf16x8, w);
       }
@@ -511,6 +522,41 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
   }
 }
 
+// One row's result from the sums of `count` pieces, part(w) apart; 16 lanes a row, `at` the lane's place among them.
+template <int RT, class Part>
+__device__ __forceinline__ void join_row(const AttentionView& v, const KvSequence& s, int r0, int r, int head, int at, int count,
+                                         Part part) {
+  const int size = v.c.head;
+  float m = -1e30f;
+  for (int w = 0; w < count; ++w) m = __builtin_fmaxf(m, part(w)[RT * size + r]);
+  float l = 0.0f;
+  floatx4 o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int w = 0; w < count; ++w) {
+    const float* p = part(w);
+    const float scale = __builtin_amdgcn_exp2f(p[RT * size + r] - m);
+    l += p[RT * size + RT + r] * scale;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int d = at * 4 + 64 * i;
+      if (d < size) o[i] += *reinterpret_cast<const floatx4*>(p + r * size + d) * scale;
+    }
+  }
+  const int i0 = (r0 + r) / v.group, g = r0 + r - i0 * v.group;
+  const int64_t at_row = (int64_t)(s.row0 + i0) * v.q_heads + head * v.group + g;
+  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d = at * 4 + 64 * i;
+    if (d < size) {
+      const uintx2 packed = {pack_bf16x2(o[i][0] * inverse, o[i][1] * inverse), pack_bf16x2(o[i][2] * inverse, o[i][3] * inverse)};
+      *reinterpret_cast<uintx2*>(v.out + at_row * size + d) = packed;
+    }
+  }
+  if (at == 0 && v.lse) v.lse[at_row] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+}
+
 // Joins the sums of the workers that share a tile, in their order; one workgroup for a tile and head.
 template <int RT>
 __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(DecodeView v) {
@@ -534,38 +580,318 @@ __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(DecodeView
   const int64_t size = (int64_t)RT * (c.head + 2);
   const float* base = v.partial + (int64_t)head * 2 * v.workers * size;
   auto part = [&](int w) { return base + (2 * w + (worker_start(total, used, w) <= from ? 1 : 0)) * size; };
-  for (int r = tid >> 4; r < rows; r += 16) {
-    float m = -1e30f;
-    for (int w = w0; w <= w1; ++w) m = __builtin_fmaxf(m, part(w)[RT * c.head + r]);
-    float l = 0.0f;
-    floatx4 o[4];
+  for (int r = tid >> 4; r < rows; r += 16)
+    join_row<RT>(v.a, sp.s, r0, r, head, tid & 15, w1 - w0 + 1, [&](int w) { return part(w0 + w); });
+}
+
+// ---- many rows for each sequence ---------------------------------------------------------------------
+//
+// A workgroup of four waves takes 128 packed rows of a sequence and cache head, 32 a wave, and goes
+// over the positions 64 at a time.  The four waves widen a stage's codes to bf16 (exact) once for all: keys as
+// [position][d], values transposed as [d][position], both in LDS, two stages taking turns with one barrier
+// each; the next stage's codes are on their way in registers.  Per wave and stage, with n = lane & 31 and h = lane >> 5:
+//   S^T = K Q^T   column n of the result is a row of q, a lane holds positions 8 j + 4 h + i
+//   O^T = V^T P^T where the values lie in LDS in that same order of positions, so the weights go from one
+//                 product into the next without leaving their lane.
+// Scales, maxima and roundings are as above.
+//
+// 16-byte pieces of a key row are stored at piece ^ (position & 15), those of a value row at
+// piece ^ ((d ^ d >> 2) & 7): eight lanes that read or write together then meet eight different places.
+//
+// Bound: matrix instructions, with the softmax's vector instructions between them.
+constexpr int kStage = 64;
+constexpr int kPromptRows = 128;
+
+struct PromptView {
+  AttentionView a;
+  float* partial;   // [slots][splits][heads][tile rows][head + 2] when splits > 1
+  int slots;        // tiles of rows, at most
+  int splits;
+  int rows_from;    // sequences with more packed rows than this are this kernel's
+};
+
+__device__ __forceinline__ int prompt_tiles(const AttentionView& v, int rows_from, int b) {
+  const int rows = kv_sequence(v.c, b).n * v.group;
+  return rows > rows_from ? (rows + kPromptRows - 1) / kPromptRows : 0;
+}
+
+template <bool F8, int DP, bool SMALL>
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_prompt_kernel(PromptView v) {
+  constexpr int RT = kPromptRows;
+  constexpr int KC = DP / 8;             // 16-byte pieces of a key row
+  constexpr int KX = KC < 16 ? KC - 1 : 15;
+  constexpr int KN = DP / 64;            // pieces of 16 codes that a lane stages of the keys
+  constexpr int VN = DP < 128 ? 1 : DP / 128;  // groups of 8 positions x 4 values that a lane stages
+  __shared__ uintx4 keys[2][kStage * KC];
+  __shared__ uintx4 vals[2][DP * 8];
+  __shared__ float kscale[2][kStage], vscale[2][kStage];
+  __shared__ int there[2][4];
+  const KvCacheView& c = v.a.c;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = lane & 31, h = lane >> 5;
+  const int head = blockIdx.x % c.heads, rest = blockIdx.x / c.heads;
+  const int split = rest % v.splits, slot = v.slots - 1 - rest / v.splits;  // the last tiles of a prompt see the most
+  int64_t index;
+  const int b = kv_find_item(c.batch, slot, lane, &index, [&](int s) { return prompt_tiles(v.a, v.rows_from, s); });
+  if (b < 0) return;
+  const KvSequence s = kv_sequence(c, b);
+  const int r0 = __builtin_amdgcn_readfirstlane((int)index) * RT, rows = min(s.n * v.a.group - r0, RT);
+  const int p_first = s.len - s.n + r0 / v.a.group, p_last = s.len - s.n + (r0 + rows - 1) / v.a.group;
+  // positions that some row of the tile sees, and that all of them see
+  const int lo = v.a.window > 0 ? max(0, p_first - v.a.window + 1) : 0;
+  const int hi = v.a.causal ? min(s.len, p_last + 1) : s.len;
+  const int all_lo = v.a.window > 0 ? max(0, p_last - v.a.window + 1) : 0;
+  const int all_hi = v.a.causal ? min(s.len, p_first + 1) : s.len;
+  const int u_first = lo / kStage, u_count = max((hi + kStage - 1) / kStage - u_first, 0);
+  const int u0 = u_first + (int)((int64_t)u_count * split / v.splits);
+  const int u1 = u_first + (int)((int64_t)u_count * (split + 1) / v.splits);
+
+  bf16x8 q[DP / 16];
+  int sees_lo, sees_hi;
+  {
+    const int r = r0 + min(wave * 32 + n, rows - 1);
+    const int i = r / v.a.group, g = r - i * v.a.group;
+    const uint16_t* qr = v.a.q + ((int64_t)(s.row0 + i) * v.a.q_heads + head * v.a.group + g) * c.head;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int w = w0; w <= w1; ++w) {
-      const float* p = part(w);
-      const float scale = __builtin_amdgcn_exp2f(p[RT * c.head + r] - m);
-      l += p[RT * c.head + RT + r] * scale;
+    for (int k = 0; k < DP / 16; ++k) q[k] = 16 * k < c.head ? *reinterpret_cast<const bf16x8*>(qr + 16 * k + 8 * h) : bf16x8{};
+    const int p = s.len - s.n + i;
+    sees_hi = v.a.causal ? min(s.len, p + 1) : s.len;
+    sees_lo = v.a.window > 0 ? max(0, p - v.a.window + 1) : 0;
+  }
+  floatx16 acc[DP / 32];
+  float top = -1e30f, sum = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int d = (tid & 15) * 4 + 64 * i;
-        if (d < c.head) o[i] += *reinterpret_cast<const floatx4*>(p + r * c.head + d) * scale;
+  for (int i = 0; i < DP / 32; ++i)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
+  const float to_log2 = 1.44269504088896341f;
+  const float cap = v.a.softcap;
+  const float factor = cap > 0.0f ? v.a.scale : v.a.scale * to_log2;
+  const int* table = c.table + (int64_t)b * c.width;
+  const int in_page = (1 << c.page_log2) - 1;
+
+  // Stage: wave w brings positions 16 w to 16 w + 15.  Keys: 16 codes a piece, lane -> (position, piece); values: lane ->
+  // (eight positions as S^T orders them, four values).
+  uintx4 kraw[KN];
+  uint32_t vraw[VN][8];
+  float scale_raw = 0.0f;
+  bool present = false;
+  const int kpos = lane / (DP / 16), kpiece = lane % (DP / 16);  // 64 / (DP / 16) positions at once
+  const int vquad = lane % (DP < 128 ? DP / 4 : 32), vhalf = DP < 128 ? (lane / (DP / 4)) & 1 : h;
+  auto page_of = [&](int u) {
+    const int j = u * kStage + 16 * wave;
+    int page = -1;
+    if (u < u1 && j < hi && j + 16 > lo) page = table[j >> c.page_log2];
+    page = __builtin_amdgcn_readfirstlane(page);
+    return (unsigned)page < (unsigned)c.pages ? page : -1;
+  };
+  auto fetch = [&](int u, int page) {
+    present = page >= 0;
+    if (!present) return;
+    const int row = (u * kStage + 16 * wave) & in_page;
+    const int64_t at = kv_row(c, page, head, row);
+    const uint8_t* kp = c.codes[0] + at;
+    const uint8_t* vp = c.codes[1] + at;
+#pragma unroll
+    for (int i = 0; i < KN; ++i)
+      kraw[i] = *reinterpret_cast<const uintx4*>(kp + (uint32_t)((i * (1024 / DP) + kpos) * c.head + min(16 * kpiece, c.head - 16)));
+#pragma unroll
+    for (int i = 0; i < VN; ++i)
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        vraw[i][e] = *reinterpret_cast<const uint32_t*>(
+            vp + (uint32_t)((8 * (e >> 2) + 4 * vhalf + (e & 3)) * c.head + min(128 * i + 4 * vquad, c.head - 4)));
+    const int64_t sc = kv_scale(c, page, head, row + (lane & 15));
+    scale_raw = c.scales[(lane >> 4) & 1][sc];
+  };
+  auto stage = [&](int u, int buf) {
+    if (!present) {
+#pragma unroll
+      for (int i = 0; i < KN; ++i) kraw[i] = uintx4{0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int i = 0; i < VN; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) vraw[i][e] = 0u;
+      scale_raw = 0.0f;
+    }
+    const int j0 = u * kStage + 16 * wave;
+    if (F8 && (j0 < lo || j0 + 16 > hi)) {
+      // positions that nobody sees may hold NaN codes, which a weight of zero does not cancel
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = j0 + 8 * (e >> 2) + 4 * vhalf + (e & 3);
+#pragma unroll
+        for (int i = 0; i < VN; ++i) vraw[i][e] = j >= lo && j < hi ? vraw[i][e] : 0u;
       }
     }
-    const int i0 = (r0 + r) / v.a.group, h = r0 + r - i0 * v.a.group;
-    const int64_t at_row = (int64_t)(sp.s.row0 + i0) * v.a.q_heads + head * v.a.group + h;
-    const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = (tid & 15) * 4 + 64 * i;
-      if (d < c.head) {
-        const uintx2 packed = {pack_bf16x2(o[i][0] * inverse, o[i][1] * inverse), pack_bf16x2(o[i][2] * inverse, o[i][3] * inverse)};
-        *reinterpret_cast<uintx2*>(v.a.out + at_row * c.head + d) = packed;
+    for (int i = 0; i < KN; ++i) {
+      const int pos = 16 * wave + i * (1024 / DP) + kpos;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uintx4 w;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          w[2 * e] = widen2<F8, 0>(kraw[i][2 * half + e]);
+          w[2 * e + 1] = widen2<F8, 2>(kraw[i][2 * half + e]);
+        }
+        keys[buf][pos * KC + ((2 * kpiece + half) ^ (pos & KX))] = w;
       }
     }
-    if ((tid & 15) == 0 && v.a.lse) v.a.lse[at_row] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      uint32_t one[8][1];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) one[e][0] = vraw[i][e];
+      static_for<0, 4>([&](auto t) {
+        const int d = 128 * i + 4 * vquad + decltype(t)::value;
+        const uintx4 w = __builtin_bit_cast(uintx4, column8<F8, decltype(t)::value>(one));
+        vals[buf][d * 8 + ((2 * wave + vhalf) ^ ((d ^ (d >> 2)) & 7))] = w;
+      });
+    }
+    float ks = scale_raw, vs = __shfl_xor(scale_raw, 16);  // lanes 0 to 15: of position 16 wave + lane
+    keep_to_its_rows(ks, vs);
+    if (lane < 16) {
+      kscale[buf][16 * wave + lane] = ks * factor;
+      vscale[buf][16 * wave + lane] = vs;
+    }
+    if (lane == 0) there[buf][wave] = present ? 1 : 0;
+  };
+
+  auto work = [&](int u, int buf, auto between) {
+    const int j0 = u * kStage;
+    floatx16 sc[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) sc[kt][e] = 0.0f;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int k = 0; k < DP / 16; ++k) {
+        const int pos = 32 * kt + n;
+        const bf16x8 a = __builtin_bit_cast(bf16x8, keys[buf][pos * KC + ((2 * k + h) ^ (pos & KX))]);
+        sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], sc[kt], 0, 0, 0);
+      }
+    between();
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        float y = sc[kt][e] * kscale[buf][32 * kt + 8 * (e >> 2) + 4 * h + (SMALL ? (e & 3) : 0)];
+        if (cap > 0.0f) {
+          const float z = __builtin_amdgcn_exp2f(y * (2.0f * to_log2 / cap));
+          y = (cap * to_log2) * (1.0f - 2.0f / (1.0f + z));
+        }
+        sc[kt][e] = y;
+      }
+    const bool gap = (there[buf][0] & there[buf][1] & there[buf][2] & there[buf][3]) == 0;
+    if (__builtin_amdgcn_readfirstlane((int)(gap || j0 < all_lo || j0 + kStage > all_hi)) != 0) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int pos = j0 + 32 * kt + 8 * (e >> 2) + 4 * h + (e & 3);
+          const bool seen = there[buf][2 * kt + (e >> 3)] != 0 && pos >= sees_lo && pos < sees_hi;
+          sc[kt][e] = seen ? sc[kt][e] : -INFINITY;
+        }
+    }
+    float most = sc[0][0];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, sc[kt][e]);
+    // the maximum in use may lag behind by up to 2^8, which f32 and bf16 weights bear
+    if (__any(most > top + 8.0f)) {
+      most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+      const float now = __builtin_fmaxf(top, most);
+      const float scale = __builtin_amdgcn_exp2f(top - now);
+      top = now;
+      sum *= scale;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) acc[i] *= scale;
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      uintx4 w;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const int r = 8 * (g & 1) + e, pos = 32 * (g >> 1) + 8 * (r >> 2) + 4 * h;
+        const float p0 = __builtin_amdgcn_exp2f(sc[g >> 1][r] - top), p1 = __builtin_amdgcn_exp2f(sc[g >> 1][r + 1] - top);
+        sum += p0 + p1;
+        w[e >> 1] = pack_bf16x2(p0 * vscale[buf][pos + (SMALL ? (r & 3) : 0)], p1 * vscale[buf][pos + (SMALL ? (r & 3) + 1 : 0)]);
+      }
+      const bf16x8 p = __builtin_bit_cast(bf16x8, w);
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        const int d = 32 * i + n;
+        const bf16x8 a = __builtin_bit_cast(bf16x8, vals[buf][d * 8 + ((2 * g + h) ^ ((d ^ (d >> 2)) & 7))]);
+        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p, acc[i], 0, 0, 0);
+      }
+    }
+  };
+
+  if (u0 < u1) {
+    fetch(u0, page_of(u0));
+    stage(u0, 0);
+    int next = page_of(u0 + 2);
+    fetch(u0 + 1, page_of(u0 + 1));
+    __syncthreads();
+    for (int u = u0; u < u1; ++u) {
+      const int buf = (u - u0) & 1;
+      work(u, buf, [&] {
+        if (u + 1 < u1) {
+          stage(u + 1, buf ^ 1);
+          fetch(u + 2, next);
+          next = page_of(u + 3);
+        }
+      });
+      __syncthreads();
+    }
+  }
+
+  const float l = sum + __shfl_xor(sum, 32);
+  const int r = wave * 32 + n;
+  if (r >= rows) return;
+  const int i = (r0 + r) / v.a.group, g = r0 + r - i * v.a.group;
+  const int64_t at_row = (int64_t)(s.row0 + i) * v.a.q_heads + head * v.a.group + g;
+  const bool joined = v.splits > 1;
+  float* part = joined ? v.partial + (((int64_t)slot * v.splits + split) * c.heads + head) * RT * (c.head + 2) : nullptr;
+  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+  for (int i2 = 0; i2 < DP / 32; ++i2)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 32 * i2 + 8 * e + 4 * h;
+      if (d >= c.head) continue;
+      const floatx4 o = {acc[i2][4 * e], acc[i2][4 * e + 1], acc[i2][4 * e + 2], acc[i2][4 * e + 3]};
+      if (joined) *reinterpret_cast<floatx4*>(part + (int64_t)r * c.head + d) = o;
+      else *reinterpret_cast<uintx2*>(v.a.out + at_row * c.head + d) =
+          uintx2{pack_bf16x2(o[0] * inverse, o[1] * inverse), pack_bf16x2(o[2] * inverse, o[3] * inverse)};
+    }
+  if (h == 0 && joined) {
+    part[(int64_t)RT * c.head + r] = top;
+    part[(int64_t)RT * c.head + RT + r] = l;
+  } else if (h == 0 && v.a.lse) {
+    v.a.lse[at_row] = l == 0.0f ? -INFINITY : (top + __builtin_log2f(l)) * 0.693147180559945309f;
   }
 }
 
+// Joins the pieces of a tile of rows; one workgroup for 16 rows of a tile and head.
+__global__ __launch_bounds__(256) void kv_cache_attention_prompt_join_kernel(PromptView v) {
+  const KvCacheView& c = v.a.c;
+  const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
+  const int slot = blockIdx.x / (kPromptRows / 16);
+  int64_t index;
+  const int b = kv_find_item(c.batch, slot, lane, &index, [&](int s) { return prompt_tiles(v.a, v.rows_from, s); });
+  if (b < 0) return;
+  const KvSequence s = kv_sequence(c, b);
+  const int r0 = (int)index * kPromptRows, r = (blockIdx.x % (kPromptRows / 16)) * 16 + (tid >> 4);
+  if (r >= min(s.n * v.a.group - r0, kPromptRows)) return;
+  const float* base = v.partial + ((int64_t)slot * v.splits * c.heads + head) * kPromptRows * (c.head + 2);
+  join_row<kPromptRows>(v.a, s, r0, r, head, tid & 15, v.splits,
+                        [&](int w) { return base + (int64_t)w * c.heads * kPromptRows * (c.head + 2); });
+}
 
 // How a call runs, from its shapes alone (lengths are device data).
 struct DecodePlan {
@@ -593,6 +919,49 @@ DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_h
   return d;
 }
 
+// Packed rows of a sequence up to which the streaming kernel takes it in calls that both kernels serve.
+constexpr int kFewRows = 64;
+
+struct PromptPlan {
+  bool used;
+  int splits;
+  int64_t slots;
+  size_t bytes;
+};
+
+PromptPlan PlanPrompt(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head, int64_t positions) {
+  PromptPlan d{};
+  const int64_t group = q_heads / kv_heads;
+  d.used = batch > 0 && rows * group > kFewRows && rows > 2 * batch;
+  if (!d.used) return d;
+  d.slots = rows * group / (kPromptRows) + batch;
+  const int64_t stages = (positions + kStage - 1) / kStage;
+  int64_t n = 512 / (d.slots * kv_heads);
+  if (n > stages / 4) n = stages / 4;
+  if (n > 16) n = 16;
+  d.splits = n < 1 ? 1 : (int)n;
+  d.bytes = d.splits > 1 ? (size_t)(d.slots * d.splits * kv_heads * kPromptRows * (head + 2)) * 4 : 0;
+  return d;
+}
+
+template <bool F8, int DP>
+void LaunchPrompt(const PromptView& v, hipStream_t stream) {
+  const unsigned grid = (unsigned)(v.slots * v.splits * v.a.c.heads);
+  if (v.a.c.block_log2 < 2) kv_cache_attention_prompt_kernel<F8, DP, true><<<grid, 256, 0, stream>>>(v);
+  else kv_cache_attention_prompt_kernel<F8, DP, false><<<grid, 256, 0, stream>>>(v);
+  if (v.splits > 1) {
+    const dim3 join((unsigned)(v.slots * (kPromptRows / 16)), (unsigned)v.a.c.heads);
+    kv_cache_attention_prompt_join_kernel<<<join, 256, 0, stream>>>(v);
+  }
+}
+
+template <bool F8>
+void LaunchPrompt(int dp, const PromptView& v, hipStream_t stream) {
+  if (dp == 64) LaunchPrompt<F8, 64>(v, stream);
+  else if (dp == 128) LaunchPrompt<F8, 128>(v, stream);
+  else LaunchPrompt<F8, 256>(v, stream);
+}
+
 template <bool F8, int DP, int QT>
 void LaunchDecode(const DecodeView& v, dim3 grid, hipStream_t stream) {
   if (v.a.c.block_log2 < 2) kv_cache_attention_decode_kernel<F8, DP, QT, true><<<grid, 256, 0, stream>>>(v);
@@ -611,7 +980,9 @@ void LaunchDecode(const DecodePlan& d, const DecodeView& v, dim3 grid, hipStream
 size_t KvCacheAttentionWorkspaceBytes(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head_size,
                                       int64_t max_positions) {
   if (rows <= 0 || batch <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_size <= 0 || max_positions <= 0) return 0;
-  return PlanDecode(rows, batch, q_heads, kv_heads, head_size, max_positions).bytes;
+  // the two kernels of a call run one after the other: their sums lie behind each other
+  return PlanDecode(rows, batch, q_heads, kv_heads, head_size, max_positions).bytes +
+         PlanPrompt(rows, batch, q_heads, kv_heads, head_size, max_positions).bytes;
 }
 
 int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) {
@@ -644,8 +1015,10 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   DecodeView dv{};
   dv.a = v;
   dv.workers = d.workers;
-  dv.rows_to = INT32_MAX;
-  if (d.split && p.workspace && p.workspace_bytes >= d.bytes) dv.partial = (float*)p.workspace;
+  PromptPlan pr = PlanPrompt(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, positions);
+  dv.rows_to = pr.used ? kFewRows : INT32_MAX;
+  const bool scratch = p.workspace && p.workspace_bytes >= d.bytes + pr.bytes;
+  if (d.split && scratch) dv.partial = (float*)p.workspace;
   const dim3 grid((unsigned)(d.workers + (v.c.rows + 63) / 64), (unsigned)v.c.heads);
   char name[64];
   const bool f8 = p.cache.cache_dtype == XLA_FFI_DataType_F8E4M3FN;
@@ -657,6 +1030,19 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
     const dim3 join((unsigned)d.tiles, (unsigned)v.c.heads);
     if (d.qt == 1) kv_cache_attention_join_kernel<16><<<join, 256, 0, stream>>>(dv);
     else kv_cache_attention_join_kernel<32><<<join, 256, 0, stream>>>(dv);
+  }
+  if (pr.used) {
+    PromptView pv{};
+    pv.a = v;
+    pv.slots = (int)pr.slots;
+    pv.splits = scratch ? pr.splits : 1;
+    pv.partial = pv.splits > 1 ? (float*)((char*)p.workspace + d.bytes) : nullptr;
+    pv.rows_from = kFewRows;
+    snprintf(name, sizeof(name), "kv_cache_attention_prompt_%s_d%d_m%d%s", f8 ? "f8" : "s8", d.dp, kPromptRows,
+             pv.splits > 1 ? "_split" : "");
+    SetLastKernel(name);
+    if (f8) LaunchPrompt<true>(d.dp, pv, stream);
+    else LaunchPrompt<false>(d.dp, pv, stream);
   }
   return CheckLaunch("kv_cache_attention");
 }

@@ -36,7 +36,7 @@ int MakeKvCacheView(const XlaAmdKvCache& p, const char* what, KvCacheView* c) {
   if (p.head_size < 16 || p.head_size > 256 || p.head_size % 16 != 0)
     return Fail(kBad, "%s: the head size must be a multiple of 16 from 16 to 256", what);
   if (p.pages < 0 || p.batch < 0 || p.table_width < 0 || p.rows < 0) return Fail(kBad, "%s: negative size", what);
-  if (p.kv_heads < 1 || p.kv_heads > 4096) return Fail(kBad, "%s: kv_heads must be 1 to 4096", what);
+  if (p.kv_heads < 1 || p.kv_heads > 1024) return Fail(kBad, "%s: kv_heads must be 1 to 1024", what);
   if (p.pages > INT32_MAX || p.rows > (1 << 24) || p.batch > (1 << 20) ||
       p.table_width > (int64_t)(INT32_MAX - 1024) / p.page_size)
     return Fail(kBad, "%s: at most 2^31 - 1 pages, 2^24 rows, 2^20 sequences and 2^31 positions", what);
