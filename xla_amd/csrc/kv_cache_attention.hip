@@ -133,9 +133,15 @@ __device__ int decode_find(const DecodeView& v, int64_t at, int lane, int64_t* b
   return -1;
 }
 
-// First unit of worker w when `total` units are cut into `workers` pieces.
-__device__ __forceinline__ int64_t worker_start(int64_t total, int workers, int w) { return total * w / workers; }
-__device__ __forceinline__ int workers_used(int64_t total, int workers) { return (int)min((int64_t)workers, total); }
+// Units that a worker takes of the line: worker w has [w * piece, (w + 1) * piece).
+__device__ __forceinline__ int64_t worker_piece(int64_t total, int workers) {
+  return (uint64_t)total < (1ull << 31) ? (int64_t)(((uint32_t)total + (uint32_t)workers - 1) / (uint32_t)workers)
+                                        : (total + workers - 1) / workers;
+}
+
+__device__ __forceinline__ int divide(int64_t x, int64_t by) {
+  return (uint64_t)x < (1ull << 31) ? (int)((uint32_t)x / (uint32_t)by) : (int)(x / by);
+}
 
 // Two codes at byte places i, i + 1 -> two bf16 in a dword, exact.
 template <bool F8, int I>
@@ -225,11 +231,10 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
     if (head == 0) clear_rows_of_nobody(v.a, 64 * (blockIdx.x - v.workers));
     return;
   }
-  const int64_t total = uniform64(decode_total<RT>(v, lane));
-  const int used = v.partial ? workers_used(total, v.workers) : v.workers;
-  if (total == 0 || (int)blockIdx.x >= used) return;
-  int64_t pos = worker_start(total, used, blockIdx.x);
-  const int64_t stop = worker_start(total, used, blockIdx.x + 1);
+  const int64_t total = uniform64(decode_total<RT>(v, lane)), piece = worker_piece(total, v.workers);
+  int64_t pos = piece * blockIdx.x;
+  if (pos >= total) return;
+  const int64_t stop = min(pos + piece, total);
   int64_t before, ignored;
   int b = decode_find<RT, false>(v, pos, lane, &before, &ignored);
   before = uniform64(before);
@@ -306,14 +311,18 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
     }
 
     const int* table = c.table + (int64_t)b * c.width;
-    auto load = [&](int j0, DecodeLoads<DP, SMALL>& x) {
+    // page numbers are read a step before the loads that need them; past the range the last page is named again
+    const int last = max(sp.hi - 1, 0);
+    auto name = [&](int j0, int (&page)[2]) {
+      if (sp.hi == 0) return;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) page[h] = table[min(j0 + 16 * h, last) >> c.page_log2];
+    };
+    auto load = [&](int j0, const int (&pages)[2], DecodeLoads<DP, SMALL>& x) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int j = j0 + 16 * h;
-        int page = -1;
-        if (j < sp.hi && j + 16 > sp.lo) page = table[j >> c.page_log2];
-        page = __builtin_amdgcn_readfirstlane(page);
-        x.there[h] = (unsigned)page < (unsigned)c.pages;
+        const int j = j0 + 16 * h, page = __builtin_amdgcn_readfirstlane(pages[h]);
+        x.there[h] = (unsigned)page < (unsigned)c.pages && j < sp.hi && j + 16 > sp.lo;
         if (x.there[h]) {
           const int row = j & in_page;
           const int64_t at = kv_row(c, page, head, row);
@@ -402,7 +411,7 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
           if (cap > 0.0f) {
             // cap * tanh(y / cap), in units of log 2
             const float z = __builtin_amdgcn_exp2f(y[e] * (2.0f * to_log2 / cap));
-            y[e] = (cap * to_log2) * (1.0f - 2.0f / (1.0f + z));
+            y[e] = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
           }
         }
         if (edge) {
@@ -448,13 +457,18 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
     const int j_end = (sp.first + u1) * kUnit;
     int j = (sp.first + u0) * kUnit + 32 * wave;
     DecodeLoads<DP, SMALL> x0, x1;
-    load(j, x0);
+    int pages[2] = {-1, -1};
+    name(j, pages);
+    load(j, pages, x0);
+    name(j + kUnit, pages);
     while (j < j_end) {
-      load(j + kUnit < j_end ? j + kUnit : 0x7fffff00, x1);
+      load(j + kUnit < j_end ? j + kUnit : 0x7fffff00, pages, x1);
+      name(j + 2 * kUnit, pages);
       step(j, x0);
       j += kUnit;
       if (j >= j_end) break;
-      load(j + kUnit < j_end ? j + kUnit : 0x7fffff00, x0);
+      load(j + kUnit < j_end ? j + kUnit : 0x7fffff00, pages, x0);
+      name(j + 2 * kUnit, pages);
       step(j, x1);
       j += kUnit;
     }
@@ -563,23 +577,21 @@ __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(DecodeView
   const KvCacheView& c = v.a.c;
   const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
   const int64_t total = decode_total<RT>(v, lane);
-  const int used = workers_used(total, v.workers);
+  const int64_t piece = worker_piece(total, v.workers);
   int64_t tiles_before, units_before;
   const int b = decode_find<RT, true>(v, blockIdx.x, lane, &tiles_before, &units_before);
   if (b < 0) return;
   const DecodeSpan sp = decode_span<RT>(v, b);
   const int tile = (int)(blockIdx.x - tiles_before);
-  const int64_t from = units_before + (int64_t)tile * sp.units, to = from + sp.units;
-  int w0 = (int)min(from * used / total, (int64_t)used - 1);
-  while (worker_start(total, used, w0 + 1) <= from) ++w0;
-  while (worker_start(total, used, w0) > from) --w0;
-  int w1 = w0;
-  while (worker_start(total, used, w1 + 1) < to) ++w1;
+  const int64_t from = units_before + (int64_t)tile * sp.units;
+  const int w0 = divide(from, piece), w1 = divide(from + sp.units - 1, piece);
   if (w0 == w1) return;  // one worker had it all
   const int r0 = tile * RT, rows = min(sp.s.n * v.a.group - r0, RT);
   const int64_t size = (int64_t)RT * (c.head + 2);
   const float* base = v.partial + (int64_t)head * 2 * v.workers * size;
-  auto part = [&](int w) { return base + (2 * w + (worker_start(total, used, w) <= from ? 1 : 0)) * size; };
+  // the first worker's range ends inside the tile, the others' begin in it
+  const int first = w0 * piece <= from ? 1 : 0;
+  auto part = [&](int w) { return base + (2 * w + (w == w0 ? first : 0)) * size; };
   for (int r = tid >> 4; r < rows; r += 16)
     join_row<RT>(v.a, sp.s, r0, r, head, tid & 15, w1 - w0 + 1, [&](int w) { return part(w0 + w); });
 }
@@ -679,14 +691,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   const int kpos = lane / (DP / 16), kpiece = lane % (DP / 16);  // 64 / (DP / 16) positions at once
   const int vquad = lane % (DP < 128 ? DP / 4 : 32), vhalf = DP < 128 ? (lane / (DP / 4)) & 1 : h;
   auto page_of = [&](int u) {
-    const int j = u * kStage + 16 * wave;
-    int page = -1;
-    if (u < u1 && j < hi && j + 16 > lo) page = table[j >> c.page_log2];
-    page = __builtin_amdgcn_readfirstlane(page);
-    return (unsigned)page < (unsigned)c.pages ? page : -1;
+    return table[min(u * kStage + 16 * wave, hi - 1) >> c.page_log2];
   };
   auto fetch = [&](int u, int page) {
-    present = page >= 0;
+    const int j = u * kStage + 16 * wave;
+    present = (unsigned)page < (unsigned)c.pages && u < u1 && j < hi && j + 16 > lo;
     if (!present) return;
     const int row = (u * kStage + 16 * wave) & in_page;
     const int64_t at = kv_row(c, page, head, row);
@@ -781,7 +790,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
         float y = sc[kt][e] * kscale[buf][32 * kt + 8 * (e >> 2) + 4 * h + (SMALL ? (e & 3) : 0)];
         if (cap > 0.0f) {
           const float z = __builtin_amdgcn_exp2f(y * (2.0f * to_log2 / cap));
-          y = (cap * to_log2) * (1.0f - 2.0f / (1.0f + z));
+          y = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
         }
         sc[kt][e] = y;
       }
@@ -893,6 +902,9 @@ __global__ __launch_bounds__(256) void kv_cache_attention_prompt_join_kernel(Pro
                         [&](int w) { return base + (int64_t)w * c.heads * kPromptRows * (c.head + 2); });
 }
 
+// Packed rows of a sequence up to which the streaming kernel takes it in calls that both kernels serve.
+constexpr int kFewRows = 64;
+
 // How a call runs, from its shapes alone (lengths are device data).
 struct DecodePlan {
   int dp, qt;       // padded head; tiles of 16 rows
@@ -902,13 +914,15 @@ struct DecodePlan {
   size_t bytes;     // of scratch for the cut tiles' sums
 };
 
-DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head, int64_t positions) {
+DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head, int64_t positions, bool few) {
   DecodePlan d;
   const int64_t group = q_heads / kv_heads;
   d.dp = head <= 64 ? 64 : head <= 128 ? 128 : 256;
   const int64_t mean = batch > 0 ? (rows + batch - 1) / batch * group : 0;
   d.qt = mean <= 16 ? 1 : 2;
   d.tiles = rows * group / (16 * d.qt) + batch;
+  const int64_t most = batch * (kFewRows / (16 * d.qt));
+  if (few && d.tiles > most) d.tiles = most;
   const int64_t units = d.tiles * ((positions + kUnit - 1) / kUnit);
   const int64_t slots = 512;
   int64_t w = (slots + kv_heads - 1) / kv_heads;
@@ -918,9 +932,6 @@ DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_h
   d.bytes = d.split ? (size_t)(kv_heads * 2 * d.workers * 16 * d.qt * (head + 2)) * 4 : 0;
   return d;
 }
-
-// Packed rows of a sequence up to which the streaming kernel takes it in calls that both kernels serve.
-constexpr int kFewRows = 64;
 
 struct PromptPlan {
   bool used;
@@ -981,8 +992,8 @@ size_t KvCacheAttentionWorkspaceBytes(int64_t rows, int64_t batch, int64_t q_hea
                                       int64_t max_positions) {
   if (rows <= 0 || batch <= 0 || kv_heads <= 0 || q_heads < kv_heads || head_size <= 0 || max_positions <= 0) return 0;
   // the two kernels of a call run one after the other: their sums lie behind each other
-  return PlanDecode(rows, batch, q_heads, kv_heads, head_size, max_positions).bytes +
-         PlanPrompt(rows, batch, q_heads, kv_heads, head_size, max_positions).bytes;
+  const PromptPlan p = PlanPrompt(rows, batch, q_heads, kv_heads, head_size, max_positions);
+  return PlanDecode(rows, batch, q_heads, kv_heads, head_size, max_positions, p.used).bytes + p.bytes;
 }
 
 int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) {
@@ -1011,11 +1022,11 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   v.causal = p.causal;
   const int64_t positions = p.cache.table_width * p.cache.page_size;
   v.window = p.window >= positions ? 0 : (int)p.window;  // every position that a causal row sees is nearer
-  const DecodePlan d = PlanDecode(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, positions);
+  const PromptPlan pr = PlanPrompt(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, positions);
+  const DecodePlan d = PlanDecode(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, positions, pr.used);
   DecodeView dv{};
   dv.a = v;
   dv.workers = d.workers;
-  PromptPlan pr = PlanPrompt(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, positions);
   dv.rows_to = pr.used ? kFewRows : INT32_MAX;
   const bool scratch = p.workspace && p.workspace_bytes >= d.bytes + pr.bytes;
   if (d.split && scratch) dv.partial = (float*)p.workspace;
