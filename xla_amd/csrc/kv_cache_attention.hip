@@ -84,53 +84,69 @@ __device__ __forceinline__ int64_t uniform64(int64_t x) {
   return (int64_t)((uint64_t)hi << 32 | lo);
 }
 
-// The units of all sequences together.
-template <int RT>
-__device__ int64_t decode_total(const DecodeView& v, int lane) {
-  int64_t sum = 0;
-  for (int b = lane; b < v.a.c.batch; b += 64) {
-    const DecodeSpan s = decode_span<RT>(v, b);
-    sum += (int64_t)s.tiles * s.units;
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) sum += shfl64(sum, lane ^ off);
-  return sum;
-}
+// Where an entry of the line lies, whose entries are units (TILES false) or tiles of rows.
+struct LineSpot {
+  int b;               // the sequence, -1 past the end
+  int64_t before;      // entries before the sequence's
+  int64_t units_before, total_units;
+};
 
-// The sequence that holds entry `at` of the line, where entries are its units (TILES false) or tiles, and how
-// many entries and units lie before it; -1 past the end.
-template <int RT, bool TILES>
-__device__ int decode_find(const DecodeView& v, int64_t at, int lane, int64_t* before, int64_t* units_before) {
-  int64_t seen = 0, seen_units = 0;
-  for (int b0 = 0; b0 < v.a.c.batch; b0 += 64) {
-    int64_t n = 0, u = 0;
-    if (b0 + lane < v.a.c.batch) {
-      const DecodeSpan s = decode_span<RT>(v, b0 + lane);
-      u = (int64_t)s.tiles * s.units;
-      n = TILES ? s.tiles : u;
+// 64 sequences at a time: lane l holds sequence b0 + l, scans over the lanes give what lies before each.  `at` is
+// asked for once the total is known.
+template <int RT, bool TILES, class At>
+__device__ LineSpot line_find(const DecodeView& v, int lane, At at) {
+  const int batch = v.a.c.batch;
+  LineSpot r{-1, 0, 0, 0};
+  auto cost = [&](int b, int64_t* tiles, int64_t* units) {
+    *tiles = *units = 0;
+    if (b < batch) {
+      const DecodeSpan s = decode_span<RT>(v, b);
+      *tiles = s.tiles;
+      *units = (int64_t)s.tiles * s.units;
     }
-    int64_t incl = n, incl_u = u;
+  };
+  auto scan = [&](int64_t x) {
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-      const int64_t t = shfl64(incl, lane - off);
-      if (lane >= off) incl += t;
-      if (TILES) {
-        const int64_t tu = shfl64(incl_u, lane - off);
-        if (lane >= off) incl_u += tu;
-      }
+      const int64_t t = shfl64(x, lane - off);
+      if (lane >= off) x += t;
     }
-    if (!TILES) incl_u = incl;
-    const unsigned long long hit = __ballot(at < seen + incl && n > 0 && at >= seen + incl - n);
+    return x;
+  };
+  int64_t tiles, units;
+  cost(lane, &tiles, &units);
+  if (batch > 64) {
+    int64_t sum = units;
+    for (int b = lane + 64; b < batch; b += 64) {
+      int64_t t, u;
+      cost(b, &t, &u);
+      sum += u;
+    }
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) sum += shfl64(sum, lane ^ off);
+    r.total_units = uniform64(sum);
+  }
+  int64_t seen = 0, seen_units = 0, want = batch > 64 ? at(r.total_units) : 0;
+  for (int b0 = 0; b0 < batch; b0 += 64) {
+    if (b0 > 0) cost(b0 + lane, &tiles, &units);
+    const int64_t upto_units = scan(units);
+    if (batch <= 64) {
+      r.total_units = uniform64(shfl64(upto_units, 63));
+      want = at(r.total_units);
+    }
+    const int64_t n = TILES ? tiles : units, upto = TILES ? scan(tiles) : upto_units;
+    const unsigned long long hit = __ballot(want < seen + upto && want >= seen + upto - n);
     if (hit != 0ull) {
       const int src = __builtin_ctzll(hit);
-      *before = seen + shfl64(incl - n, src);
-      *units_before = seen_units + shfl64(incl_u - u, src);
-      return __builtin_amdgcn_readfirstlane(b0 + src);
+      r.b = __builtin_amdgcn_readfirstlane(b0 + src);
+      r.before = seen + uniform64(shfl64(upto - n, src));
+      r.units_before = seen_units + uniform64(shfl64(upto_units - units, src));
+      return r;
     }
-    seen += shfl64(incl, 63);
-    seen_units += shfl64(incl_u, 63);
+    seen += uniform64(shfl64(upto, 63));
+    seen_units += uniform64(shfl64(upto_units, 63));
   }
-  return -1;
+  return r;
 }
 
 // Units that a worker takes of the line: worker w has [w * piece, (w + 1) * piece).
@@ -154,25 +170,32 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w) {
   }
 }
 
-// Byte t of eight keys (word W = t / 4 of each) -> eight bf16.
+// Bytes T and T + 1 (T even; word T / 4) of eight keys -> eight bf16 each.
 template <bool F8, int T, int N>
-__device__ __forceinline__ bf16x8 column8(const uint32_t (&k)[8][N]) {
+__device__ __forceinline__ void columns(const uint32_t (&k)[8][N], bf16x8& first, bf16x8& second) {
   constexpr int W = T >> 2, I = T & 3;
-  uintx4 r;
+  uintx4 r, t;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const uint32_t a = k[2 * p][W], b = k[2 * p + 1][W];
     if constexpr (F8) {
-      // bytes I of both keys in the low half, where the conversion reads them
-      const uint32_t pair = __builtin_amdgcn_perm(b, a, 0x0c0c0000u | ((4 + I) << 8) | I);
-      r[p] = widen2<true, 0>(pair);
+      // byte I of both keys, then byte I + 1 of both, as the conversion reads them
+      const uint32_t pairs = __builtin_amdgcn_perm(b, a, 0x05010400u + 0x01010101u * I);
+      r[p] = widen2<true, 0>(pairs);
+      t[p] = widen2<true, 2>(pairs);
     } else {
       const float x = (float)(int8_t)(a >> (8 * I)), y = (float)(int8_t)(b >> (8 * I));
+      const float z = (float)(int8_t)(a >> (8 * I + 8)), w = (float)(int8_t)(b >> (8 * I + 8));
       r[p] = __builtin_amdgcn_perm(f32_to_bits(y), f32_to_bits(x), 0x07060302u);
+      t[p] = __builtin_amdgcn_perm(f32_to_bits(w), f32_to_bits(z), 0x07060302u);
     }
   }
-  return __builtin_bit_cast(bf16x8, r);
+  first = __builtin_bit_cast(bf16x8, r);
+  second = __builtin_bit_cast(bf16x8, t);
 }
+
+// Keeps what follows in its branch: work that few steps need is not done by all of them and thrown away.
+#define KV_CACHE_RARE() asm volatile("")
 
 // Rows first to first + 63, where they belong to no sequence: 0, lse -infinity.
 __device__ void clear_rows_of_nobody(const AttentionView& v, int first) {
@@ -216,7 +239,7 @@ struct DecodeLoads {
 };
 
 template <bool F8, int DP, int QT, bool SMALL>
-__global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeView v) {
+__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_decode_kernel(DecodeView v) {
   constexpr int RT = 16 * QT;        // packed rows of a tile
   constexpr int KW = DP / 64;        // 16-byte pieces of a key row that a lane holds
   constexpr int VT = DP / 16;        // values of a position that a lane holds
@@ -231,13 +254,14 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
     if (head == 0) clear_rows_of_nobody(v.a, 64 * (blockIdx.x - v.workers));
     return;
   }
-  const int64_t total = uniform64(decode_total<RT>(v, lane)), piece = worker_piece(total, v.workers);
-  int64_t pos = piece * blockIdx.x;
-  if (pos >= total) return;
-  const int64_t stop = min(pos + piece, total);
-  int64_t before, ignored;
-  int b = decode_find<RT, false>(v, pos, lane, &before, &ignored);
-  before = uniform64(before);
+  int64_t piece = 1;
+  const LineSpot spot = line_find<RT, false>(v, lane, [&](int64_t total) {
+    piece = worker_piece(total, v.workers);
+    return piece * blockIdx.x;
+  });
+  int64_t pos = piece * blockIdx.x, before = spot.before;
+  const int64_t stop = min(pos + piece, spot.total_units);
+  int b = spot.b;
 
   // byte offsets of a lane inside 16 rows of a page and head; a head shorter than DP repeats its end, which
   // q's zeros cancel on one side and the results beyond it are dropped on the other
@@ -311,68 +335,59 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
     }
 
     const int* table = c.table + (int64_t)b * c.width;
-    // page numbers are read a step before the loads that need them; past the range the last page is named again
+    // page numbers are read a step before the loads that need them
     const int last = max(sp.hi - 1, 0);
     auto name = [&](int j0, int (&page)[2]) {
-      if (sp.hi == 0) return;
 #pragma unroll
       for (int h = 0; h < 2; ++h) page[h] = table[min(j0 + 16 * h, last) >> c.page_log2];
     };
+    // 16 positions that no row sees, or that have no page, are read from page 0 and masked
     auto load = [&](int j0, const int (&pages)[2], DecodeLoads<DP, SMALL>& x) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int j = j0 + 16 * h, page = __builtin_amdgcn_readfirstlane(pages[h]);
-        x.there[h] = (unsigned)page < (unsigned)c.pages && j < sp.hi && j + 16 > sp.lo;
-        if (x.there[h]) {
-          const int row = j & in_page;
-          const int64_t at = kv_row(c, page, head, row);
-          const uint8_t* kp = c.codes[0] + at;
-          const uint8_t* vp = c.codes[1] + at;
+        const int j = j0 + 16 * h, named = __builtin_amdgcn_readfirstlane(pages[h]);
+        x.there[h] = (unsigned)named < (unsigned)c.pages && j < sp.hi && j + 16 > sp.lo;
+        const int page = x.there[h] ? named : 0, row = j & in_page;
+        const int64_t at = kv_row(c, page, head, row);
+        const uint8_t* kp = c.codes[0] + at;
+        const uint8_t* vp = c.codes[1] + at;
 #pragma unroll
-          for (int s = 0; s < KW; ++s) x.k[h][s] = *reinterpret_cast<const uintx4*>(kp + koff[s]);
+        for (int s = 0; s < KW; ++s) x.k[h][s] = *reinterpret_cast<const uintx4*>(kp + koff[s]);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint8_t* p = vp + voff[i];
-            if constexpr (DP == 64) {
-              x.v[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(p);
-            } else if constexpr (DP == 128) {
-              const uintx2 w = *reinterpret_cast<const uintx2*>(p);
-              x.v[4 * h + i][0] = w[0];
-              x.v[4 * h + i][1] = w[1];
-            } else {
-              const uintx4 w = *reinterpret_cast<const uintx4*>(p);
+        for (int i = 0; i < 4; ++i) {
+          const uint8_t* p = vp + voff[i];
+          if constexpr (DP == 64) {
+            x.v[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(p);
+          } else if constexpr (DP == 128) {
+            const uintx2 w = *reinterpret_cast<const uintx2*>(p);
+            x.v[4 * h + i][0] = w[0];
+            x.v[4 * h + i][1] = w[1];
+          } else {
+            const uintx4 w = *reinterpret_cast<const uintx4*>(p);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x.v[4 * h + i][e] = w[e];
-            }
+            for (int e = 0; e < 4; ++e) x.v[4 * h + i][e] = w[e];
           }
-          const int64_t sc = kv_scale(c, page, head, 0);
+        }
+        const int64_t sc = kv_scale(c, page, head, 0);
 #pragma unroll
-          for (int i = 0; i < DecodeLoads<DP, SMALL>::S; ++i) {
-            const int o = (row + 4 * grp + i) >> c.block_log2;
-            x.ks[h][i] = c.scales[0][sc + o];
-            x.vs[h][i] = c.scales[1][sc + o];
-          }
-        } else {
-#pragma unroll
-          for (int s = 0; s < KW; ++s) x.k[h][s] = uintx4{0u, 0u, 0u, 0u};
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int e = 0; e < KW; ++e) x.v[4 * h + i][e] = 0u;
-#pragma unroll
-          for (int i = 0; i < DecodeLoads<DP, SMALL>::S; ++i) x.ks[h][i] = x.vs[h][i] = 0.0f;
+        for (int i = 0; i < DecodeLoads<DP, SMALL>::S; ++i) {
+          const int o = (row + 4 * grp + i) >> c.block_log2;
+          x.ks[h][i] = c.scales[0][sc + o];
+          x.vs[h][i] = c.scales[1][sc + o];
         }
       }
     };
     auto step = [&](int j0, DecodeLoads<DP, SMALL>& x) {
+      __builtin_amdgcn_sched_barrier(0);
       if (!x.there[0] && !x.there[1]) return;
       const bool edge = j0 < all_lo || j0 + 32 > all_hi || !x.there[0] || !x.there[1];
-      if (F8 && (j0 < sp.lo || j0 + 32 > sp.hi)) {
+      if (F8 && (j0 < sp.lo || j0 + 32 > sp.hi || !x.there[0] || !x.there[1])) {
+        KV_CACHE_RARE();
         // positions that nobody sees may hold NaN codes, which a weight of zero does not cancel
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = j0 + 16 * (e >> 2) + 4 * grp + (e & 3);
-          const bool keep = j >= sp.lo && j < sp.hi;
+          const bool keep = x.there[e >> 2] && j >= sp.lo && j < sp.hi;
 #pragma unroll
           for (int w = 0; w < KW; ++w) x.v[e][w] = keep ? x.v[e][w] : 0u;
         }
@@ -399,6 +414,8 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
           const bf16x8 kk = __builtin_bit_cast(bf16x8, w);
 #pragma unroll
           for (int t = 0; t < QT; ++t) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[t][m], s[t][h], 0, 0, 0);
+          // one piece widened while the one before is multiplied, and no more of them in registers
+          __builtin_amdgcn_sched_barrier(0);
         }
       bf16x8 p[QT];
 #pragma unroll
@@ -408,13 +425,18 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
         for (int e = 0; e < 8; ++e) {
           const int h = e >> 2, i = SMALL ? (e & 3) : 0;
           y[e] = s[t][h][e & 3] * (x.ks[h][i] * factor);
-          if (cap > 0.0f) {
-            // cap * tanh(y / cap), in units of log 2
+        }
+        if (cap > 0.0f) {
+          KV_CACHE_RARE();
+          // cap * tanh(y / cap), in units of log 2
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
             const float z = __builtin_amdgcn_exp2f(y[e] * (2.0f * to_log2 / cap));
             y[e] = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
           }
         }
         if (edge) {
+          KV_CACHE_RARE();
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int j = j0 + 16 * (e >> 2) + 4 * grp + (e & 3);
@@ -446,31 +468,41 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
         }
         p[t] = __builtin_bit_cast(bf16x8, w);
       }
-      static_for<0, VT>([&](auto i) {
-        const bf16x8 vv = column8<F8, decltype(i)::value>(x.v);
+      static_for<0, VT / 2>([&](auto i) {
+        constexpr int I = 2 * decltype(i)::value;
+        bf16x8 va, vb;
+        columns<F8, I>(x.v, va, vb);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[t], acc[t][i], 0, 0, 0);
+        for (int t = 0; t < QT; ++t) {
+          acc[t][I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p[t], acc[t][I], 0, 0, 0);
+          acc[t][I + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p[t], acc[t][I + 1], 0, 0, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       });
     };
 
     // two sets of loads take turns: the next 32 positions are under way while these are worked on
     const int j_end = (sp.first + u1) * kUnit;
     int j = (sp.first + u0) * kUnit + 32 * wave;
-    DecodeLoads<DP, SMALL> x0, x1;
-    int pages[2] = {-1, -1};
-    name(j, pages);
-    load(j, pages, x0);
-    name(j + kUnit, pages);
-    while (j < j_end) {
-      load(j + kUnit < j_end ? j + kUnit : 0x7fffff00, pages, x1);
-      name(j + 2 * kUnit, pages);
-      step(j, x0);
-      j += kUnit;
-      if (j >= j_end) break;
-      load(j + kUnit < j_end ? j + kUnit : 0x7fffff00, pages, x0);
-      name(j + 2 * kUnit, pages);
-      step(j, x1);
-      j += kUnit;
+    // (past the end of the range the loads name its last positions again: no load depends on a branch, so
+    // none of its uses is drawn up to it)
+    if (sp.hi > 0 && j < j_end) {
+      DecodeLoads<DP, SMALL> x0, x1;
+      int pages[2];
+      const int j_last = j_end - kUnit + 32 * wave;
+      name(j, pages);
+      load(j, pages, x0);
+      name(min(j + kUnit, j_last), pages);
+      while (true) {
+        load(min(j + kUnit, j_last), pages, x1);
+        name(min(j + 2 * kUnit, j_last), pages);
+        step(j, x0);
+        if ((j += kUnit) >= j_end) break;
+        load(min(j + kUnit, j_last), pages, x0);
+        name(min(j + 2 * kUnit, j_last), pages);
+        step(j, x1);
+        if ((j += kUnit) >= j_end) break;
+      }
     }
 
     // the four waves' sums, 16 rows at a time
@@ -536,64 +568,62 @@ __global__ __launch_bounds__(256) void kv_cache_attention_decode_kernel(DecodeVi
   }
 }
 
-// One row's result from the sums of `count` pieces, part(w) apart; 16 lanes a row, `at` the lane's place among them.
+// One row's result from the sums of `count` pieces, part(w) apart; a wave for a row.  The lanes first hold a piece's
+// maximum and sum each, then go along the head, all pieces' sums under way together.
 template <int RT, class Part>
-__device__ __forceinline__ void join_row(const AttentionView& v, const KvSequence& s, int r0, int r, int head, int at, int count,
+__device__ __forceinline__ void join_row(const AttentionView& v, const KvSequence& s, int r0, int r, int head, int lane, int count,
                                          Part part) {
   const int size = v.c.head;
   float m = -1e30f;
-  for (int w = 0; w < count; ++w) m = __builtin_fmaxf(m, part(w)[RT * size + r]);
+  for (int w = lane; w < count; w += 64) m = __builtin_fmaxf(m, part(w)[RT * size + r]);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, off));
   float l = 0.0f;
-  floatx4 o[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int w = 0; w < count; ++w) {
-    const float* p = part(w);
-    const float scale = __builtin_amdgcn_exp2f(p[RT * size + r] - m);
-    l += p[RT * size + RT + r] * scale;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = at * 4 + 64 * i;
-      if (d < size) o[i] += *reinterpret_cast<const floatx4*>(p + r * size + d) * scale;
+  floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  const int d = min(4 * lane, size - 4);
+  for (int w0 = 0; w0 < count; w0 += 64) {
+    const int here = min(count - w0, 64);
+    float scale = 0.0f;
+    if (lane < here) {
+      const float* p = part(w0 + lane) + RT * size + r;
+      scale = __builtin_amdgcn_exp2f(p[0] - m);
+      l += p[RT] * scale;
     }
+#pragma unroll 4
+    for (int w = 0; w < here; ++w) o += *reinterpret_cast<const floatx4*>(part(w0 + w) + (int64_t)r * size + d) * __shfl(scale, w);
   }
-  const int i0 = (r0 + r) / v.group, g = r0 + r - i0 * v.group;
-  const int64_t at_row = (int64_t)(s.row0 + i0) * v.q_heads + head * v.group + g;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
+  const int i = (r0 + r) / v.group, g = r0 + r - i * v.group;
+  const int64_t at_row = (int64_t)(s.row0 + i) * v.q_heads + head * v.group + g;
   const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int d = at * 4 + 64 * i;
-    if (d < size) {
-      const uintx2 packed = {pack_bf16x2(o[i][0] * inverse, o[i][1] * inverse), pack_bf16x2(o[i][2] * inverse, o[i][3] * inverse)};
-      *reinterpret_cast<uintx2*>(v.out + at_row * size + d) = packed;
-    }
-  }
-  if (at == 0 && v.lse) v.lse[at_row] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.693147180559945309f;
+  if (4 * lane < size)
+    *reinterpret_cast<uintx2*>(v.out + at_row * size + d) =
+        uintx2{pack_bf16x2(o[0] * inverse, o[1] * inverse), pack_bf16x2(o[2] * inverse, o[3] * inverse)};
+  if (lane == 0 && v.lse) v.lse[at_row] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.693147180559945309f;
 }
 
-// Joins the sums of the workers that share a tile, in their order; one workgroup for a tile and head.
+// Joins the sums of the workers that share a tile, in their order; a workgroup for four rows of a tile and head.
 template <int RT>
 __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(DecodeView v) {
   const KvCacheView& c = v.a.c;
-  const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
-  const int64_t total = decode_total<RT>(v, lane);
-  const int64_t piece = worker_piece(total, v.workers);
-  int64_t tiles_before, units_before;
-  const int b = decode_find<RT, true>(v, blockIdx.x, lane, &tiles_before, &units_before);
-  if (b < 0) return;
-  const DecodeSpan sp = decode_span<RT>(v, b);
-  const int tile = (int)(blockIdx.x - tiles_before);
-  const int64_t from = units_before + (int64_t)tile * sp.units;
+  const int lane = threadIdx.x & 63, head = blockIdx.y, at = blockIdx.x / (RT / 4);
+  const int r = (blockIdx.x % (RT / 4)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const LineSpot spot = line_find<RT, true>(v, lane, [&](int64_t) { return (int64_t)at; });
+  if (spot.b < 0) return;
+  const int64_t piece = worker_piece(spot.total_units, v.workers);
+  const DecodeSpan sp = decode_span<RT>(v, spot.b);
+  const int tile = (int)(at - spot.before), r0 = tile * RT;
+  if (r >= sp.s.n * v.a.group - r0) return;
+  const int64_t from = spot.units_before + (int64_t)tile * sp.units;
   const int w0 = divide(from, piece), w1 = divide(from + sp.units - 1, piece);
   if (w0 == w1) return;  // one worker had it all
-  const int r0 = tile * RT, rows = min(sp.s.n * v.a.group - r0, RT);
   const int64_t size = (int64_t)RT * (c.head + 2);
   const float* base = v.partial + (int64_t)head * 2 * v.workers * size;
   // the first worker's range ends inside the tile, the others' begin in it
   const int first = w0 * piece <= from ? 1 : 0;
-  auto part = [&](int w) { return base + (2 * w + (w == w0 ? first : 0)) * size; };
-  for (int r = tid >> 4; r < rows; r += 16)
-    join_row<RT>(v.a, sp.s, r0, r, head, tid & 15, w1 - w0 + 1, [&](int w) { return part(w0 + w); });
+  join_row<RT>(v.a, sp.s, r0, r, head, lane, w1 - w0 + 1,
+               [&](int w) { return base + (2 * (w0 + w) + (w == 0 ? first : 0)) * size; });
 }
 
 // ---- many rows for each sequence ---------------------------------------------------------------------
@@ -696,7 +726,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   auto fetch = [&](int u, int page) {
     const int j = u * kStage + 16 * wave;
     present = (unsigned)page < (unsigned)c.pages && u < u1 && j < hi && j + 16 > lo;
-    if (!present) return;
+    page = present ? page : 0;  // read, and masked
     const int row = (u * kStage + 16 * wave) & in_page;
     const int64_t at = kv_row(c, page, head, row);
     const uint8_t* kp = c.codes[0] + at;
@@ -714,23 +744,15 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     scale_raw = c.scales[(lane >> 4) & 1][sc];
   };
   auto stage = [&](int u, int buf) {
-    if (!present) {
-#pragma unroll
-      for (int i = 0; i < KN; ++i) kraw[i] = uintx4{0u, 0u, 0u, 0u};
-#pragma unroll
-      for (int i = 0; i < VN; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) vraw[i][e] = 0u;
-      scale_raw = 0.0f;
-    }
     const int j0 = u * kStage + 16 * wave;
-    if (F8 && (j0 < lo || j0 + 16 > hi)) {
+    if (F8 && (!present || j0 < lo || j0 + 16 > hi)) {
+      KV_CACHE_RARE();
       // positions that nobody sees may hold NaN codes, which a weight of zero does not cancel
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const int j = j0 + 8 * (e >> 2) + 4 * vhalf + (e & 3);
 #pragma unroll
-        for (int i = 0; i < VN; ++i) vraw[i][e] = j >= lo && j < hi ? vraw[i][e] : 0u;
+        for (int i = 0; i < VN; ++i) vraw[i][e] = present && j >= lo && j < hi ? vraw[i][e] : 0u;
       }
     }
 #pragma unroll
@@ -752,10 +774,12 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
       uint32_t one[8][1];
 #pragma unroll
       for (int e = 0; e < 8; ++e) one[e][0] = vraw[i][e];
-      static_for<0, 4>([&](auto t) {
-        const int d = 128 * i + 4 * vquad + decltype(t)::value;
-        const uintx4 w = __builtin_bit_cast(uintx4, column8<F8, decltype(t)::value>(one));
-        vals[buf][d * 8 + ((2 * wave + vhalf) ^ ((d ^ (d >> 2)) & 7))] = w;
+      static_for<0, 2>([&](auto t) {
+        const int d = 128 * i + 4 * vquad + 2 * decltype(t)::value;
+        bf16x8 va, vb;
+        columns<F8, 2 * decltype(t)::value>(one, va, vb);
+        vals[buf][d * 8 + ((2 * wave + vhalf) ^ ((d ^ (d >> 2)) & 7))] = __builtin_bit_cast(uintx4, va);
+        vals[buf][d * 8 + 8 + ((2 * wave + vhalf) ^ (((d + 1) ^ (d >> 2)) & 7))] = __builtin_bit_cast(uintx4, vb);
       });
     }
     float ks = scale_raw, vs = __shfl_xor(scale_raw, 16);  // lanes 0 to 15: of position 16 wave + lane
@@ -886,19 +910,19 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   }
 }
 
-// Joins the pieces of a tile of rows; one workgroup for 16 rows of a tile and head.
+// Joins the pieces of a tile of rows; a workgroup for four rows of a tile and head.
 __global__ __launch_bounds__(256) void kv_cache_attention_prompt_join_kernel(PromptView v) {
   const KvCacheView& c = v.a.c;
-  const int tid = threadIdx.x, lane = tid & 63, head = blockIdx.y;
-  const int slot = blockIdx.x / (kPromptRows / 16);
+  const int lane = threadIdx.x & 63, head = blockIdx.y, slot = blockIdx.x / (kPromptRows / 4);
   int64_t index;
   const int b = kv_find_item(c.batch, slot, lane, &index, [&](int s) { return prompt_tiles(v.a, v.rows_from, s); });
   if (b < 0) return;
   const KvSequence s = kv_sequence(c, b);
-  const int r0 = (int)index * kPromptRows, r = (blockIdx.x % (kPromptRows / 16)) * 16 + (tid >> 4);
+  const int r0 = (int)index * kPromptRows;
+  const int r = (blockIdx.x % (kPromptRows / 4)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (r >= min(s.n * v.a.group - r0, kPromptRows)) return;
   const float* base = v.partial + ((int64_t)slot * v.splits * c.heads + head) * kPromptRows * (c.head + 2);
-  join_row<kPromptRows>(v.a, s, r0, r, head, tid & 15, v.splits,
+  join_row<kPromptRows>(v.a, s, r0, r, head, lane, v.splits,
                         [&](int w) { return base + (int64_t)w * c.heads * kPromptRows * (c.head + 2); });
 }
 
@@ -961,7 +985,7 @@ void LaunchPrompt(const PromptView& v, hipStream_t stream) {
   if (v.a.c.block_log2 < 2) kv_cache_attention_prompt_kernel<F8, DP, true><<<grid, 256, 0, stream>>>(v);
   else kv_cache_attention_prompt_kernel<F8, DP, false><<<grid, 256, 0, stream>>>(v);
   if (v.splits > 1) {
-    const dim3 join((unsigned)(v.slots * (kPromptRows / 16)), (unsigned)v.a.c.heads);
+    const dim3 join((unsigned)(v.slots * (kPromptRows / 4)), (unsigned)v.a.c.heads);
     kv_cache_attention_prompt_join_kernel<<<join, 256, 0, stream>>>(v);
   }
 }
@@ -1038,7 +1062,7 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   if (f8) LaunchDecode<true>(d, dv, grid, stream);
   else LaunchDecode<false>(d, dv, grid, stream);
   if (dv.partial) {
-    const dim3 join((unsigned)d.tiles, (unsigned)v.c.heads);
+    const dim3 join((unsigned)(d.tiles * 4 * d.qt), (unsigned)v.c.heads);
     if (d.qt == 1) kv_cache_attention_join_kernel<16><<<join, 256, 0, stream>>>(dv);
     else kv_cache_attention_join_kernel<32><<<join, 256, 0, stream>>>(dv);
   }

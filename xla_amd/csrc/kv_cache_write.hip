@@ -63,7 +63,7 @@ int MakeKvCacheView(const XlaAmdKvCache& p, const char* what, KvCacheView* c) {
   c->page_log2 = page_log2;
   c->block_log2 = block_log2;
   c->batch = (int)p.batch;
-  c->width = (int)p.table_width;
+  c->width = p.pages > 0 ? (int)p.table_width : 0;  // without pages no position exists
   c->rows = (int)p.rows;
   return 0;
 }
