@@ -11,6 +11,11 @@
 
 namespace xla_amd {
 
+// Integers that no kernel writes while another reads them: a read whose index is the same in all lanes goes through
+// the scalar cache, also behind stores and loads to LDS.
+typedef const __attribute__((address_space(4))) int* const_ints_t;
+static __device__ __forceinline__ int const_int(const int* p, int64_t i) { return ((const_ints_t)(uintptr_t)p)[i]; }
+
 struct KvCacheView {
   uint8_t* codes[2];  // k, v: [pages, heads, page, head]
   float* scales[2];   // [pages, heads, page / block]
@@ -31,15 +36,15 @@ struct KvSequence {
 
 static __device__ __forceinline__ KvSequence kv_sequence(const KvCacheView& c, int b) {
   KvSequence s;
-  s.row0 = min(max(c.offsets[b], 0), c.rows);
-  s.n = min(max(c.offsets[b + 1], s.row0), c.rows) - s.row0;
-  s.len = min(max(c.lens[b], 0), c.width << c.page_log2);
+  s.row0 = min(max(const_int(c.offsets, b), 0), c.rows);
+  s.n = min(max(const_int(c.offsets, b + 1), s.row0), c.rows) - s.row0;
+  s.len = min(max(const_int(c.lens, b), 0), c.width << c.page_log2);
   return s;
 }
 
 // The page that holds position `pos` of sequence b, or -1 where the table names none.
 static __device__ __forceinline__ int kv_page(const KvCacheView& c, int b, int pos) {
-  const int page = c.table[(int64_t)b * c.width + (pos >> c.page_log2)];
+  const int page = const_int(c.table, (int64_t)b * c.width + (pos >> c.page_log2));
   return (unsigned)page < (unsigned)c.pages ? page : -1;
 }
 
@@ -49,6 +54,19 @@ static __device__ __forceinline__ int64_t kv_row(const KvCacheView& c, int page,
 }
 static __device__ __forceinline__ int64_t kv_scale(const KvCacheView& c, int page, int head, int row) {
   return (((int64_t)page * c.heads + head) << (c.page_log2 - c.block_log2)) + (row >> c.block_log2);
+}
+
+__device__ __forceinline__ int64_t uniform64(int64_t x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uint64_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
+// Descriptor of `bytes` bytes from base (the same in all lanes) on: loads past them, all of them where bytes is 0,
+// return 0.
+static __device__ __forceinline__ __amdgpu_buffer_rsrc_t kv_rsrc(const void* base, int bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(uniform64((int64_t)(uintptr_t)base)), 0,
+                                           __builtin_amdgcn_readfirstlane(bytes), 0x00020000);
 }
 
 // Finds item `item` of a ragged call by itself: sequence b has cost(b) items, in order.  64 sequences at a

@@ -78,12 +78,6 @@ __device__ __forceinline__ int64_t shfl64(int64_t x, int src) {
   return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
 }
 
-__device__ __forceinline__ int64_t uniform64(int64_t x) {
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)(uint64_t)x);
-  const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)((uint64_t)x >> 32));
-  return (int64_t)((uint64_t)hi << 32 | lo);
-}
-
 // Where an entry of the line lies, whose entries are units (TILES false) or tiles of rows.
 struct LineSpot {
   int b;               // the sequence, -1 past the end
@@ -170,6 +164,12 @@ __device__ __forceinline__ uint32_t widen2(uint32_t w) {
   }
 }
 
+// Eight codes -> eight bf16.
+template <bool F8>
+__device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi) {
+  return __builtin_bit_cast(bf16x8, uintx4{widen2<F8, 0>(lo), widen2<F8, 2>(lo), widen2<F8, 0>(hi), widen2<F8, 2>(hi)});
+}
+
 // Bytes T and T + 1 (T even; word T / 4) of eight keys -> eight bf16 each.
 template <bool F8, int T, int N>
 __device__ __forceinline__ void columns(const uint32_t (&k)[8][N], bf16x8& first, bf16x8& second) {
@@ -195,6 +195,7 @@ __device__ __forceinline__ void columns(const uint32_t (&k)[8][N], bf16x8& first
 }
 
 // Keeps what follows in its branch: work that few steps need is not done by all of them and thrown away.
+#define KV_CACHE_INLINE __attribute__((always_inline))  // of a lambda: its captures stay in registers
 #define KV_CACHE_RARE() asm volatile("")
 
 // Rows first to first + 63, where they belong to no sequence: 0, lse -infinity.
@@ -228,23 +229,42 @@ __device__ __forceinline__ void keep_to_its_rows(float& key_scale, float& value_
   }
 }
 
-// What a wave has under way for 32 positions: key and value codes of both 16s, and their scales.
-template <int DP, bool SMALL>
-struct DecodeLoads {
-  static constexpr int S = SMALL ? 4 : 1;
-  uintx4 k[2][DP / 64];
-  uint32_t v[8][DP / 64];
-  float ks[2][S], vs[2][S];
-  bool there[2];
-};
+typedef __attribute__((address_space(3))) void* lds_ptr_t;
+typedef int intx2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) intx2* lds_tr_ptr_t;
+
+// (functions of their own: inside a lambda these builtins cost the kernel its launch stub)
+// 64 lanes x 16 bytes into 1 KiB of LDS from `to` on, in the order of the lanes; past the buffer's end zeros.
+__device__ __forceinline__ void load16_to_lds(__amdgpu_buffer_rsrc_t r, uint8_t* to, uint32_t from) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr_t)to, 16, from, 0, 0, 0);
+}
+// 64 lanes x 4 bytes, each lane from an address of its own.
+__device__ __forceinline__ void load4_to_lds(const char* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from, (lds_ptr_t)to, 4, 0, 0);
+}
+// In every 16 lanes: lane i points at 8 bytes of row i / 2, the even lanes at one octet, the odd ones at the next;
+// lane j receives byte j of the eight rows.
+__device__ __forceinline__ intx2 read_columns(const uint8_t* from) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_tr_ptr_t)from);
+}
+
+// A wave's ring in LDS: each slot holds 32 positions as they lie in the pages, keys and values, and 64 scales.
+constexpr int decode_depth(int dp) { return dp == 64 ? 3 : 2; }
+constexpr int decode_slot(int dp) { return 64 * dp + 256; }
+constexpr int decode_residents(int dp) { return dp == 256 ? 1 : 2; }  // workgroups that share a CU
 
 template <bool F8, int DP, int QT, bool SMALL>
-__global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_decode_kernel(DecodeView v) {
+__global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_decode_kernel(DecodeView v) {
   constexpr int RT = 16 * QT;        // packed rows of a tile
-  constexpr int KW = DP / 64;        // 16-byte pieces of a key row that a lane holds
-  constexpr int VT = DP / 16;        // values of a position that a lane holds
+  constexpr int NI = DP / 64;        // 1024-byte loads for 16 positions; 16-byte pieces of a key row in a lane
+  constexpr int VT = DP / 16;        // matrix tiles along the head
+  constexpr int NC = DP / 16;        // 16-byte pieces of a row in LDS
+  constexpr int KX = NC < 8 ? NC - 1 : 7;
   constexpr int NF = DP + 4;         // row stride of the sums in LDS
-  __shared__ float sums[4][16 * NF];
+  constexpr int S = SMALL ? 4 : 1;   // scales of four neighbouring positions
+  constexpr int DEPTH = decode_depth(DP), SLOT = decode_slot(DP), PER = 4 * NI + 1;
+  static_assert(4 * 16 * NF * 4 <= 4 * DEPTH * SLOT, "the sums take the ring's place");
+  __shared__ __attribute__((aligned(1024))) uint8_t ring[4 * DEPTH * SLOT];
   __shared__ float tops[4][RT], totals[4][RT];
   const KvCacheView& c = v.a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -263,14 +283,24 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
   const int64_t stop = min(pos + piece, spot.total_units);
   int b = spot.b;
 
-  // byte offsets of a lane inside 16 rows of a page and head; a head shorter than DP repeats its end, which
-  // q's zeros cancel on one side and the results beyond it are dropped on the other
+  // Where a lane's 16 bytes of a load come from: LDS is filled in order, so the pieces of a row are exchanged at the
+  // source.  Keys: piece ^ (row & 7), met again when 16 rows are read a piece at a time; values: piece ^ (row & 3, and
+  // 4 for the second 16 rows), when eight rows are read transposed.  A head shorter than DP repeats its end, which q's
+  // zeros cancel on one side and the results beyond it are dropped on the other.
   const int stride = c.head;
-  uint32_t koff[KW], voff[4];
+  uint32_t kfrom[NI], vfrom[2][NI];
 #pragma unroll
-  for (int s = 0; s < KW; ++s) koff[s] = (uint32_t)(col * stride + min(grp * (DP / 4) + 16 * s, stride - 16));
+  for (int i = 0; i < NI; ++i) {
+    const int r = (64 * i + lane) / NC, q = (64 * i + lane) % NC;
+    kfrom[i] = (uint32_t)(r * stride + min(16 * (q ^ (r & KX)), stride - 16));
 #pragma unroll
-  for (int i = 0; i < 4; ++i) voff[i] = (uint32_t)((4 * grp + i) * stride + min(col * VT, stride - VT));
+    for (int h = 0; h < 2; ++h) vfrom[h][i] = (uint32_t)(r * stride + min(16 * (q ^ (((r & 3) + 4 * h) & KX)), stride - 16));
+  }
+  uint8_t* const mine = ring + wave * DEPTH * SLOT;
+  const int kread = col * DP + ((NI * grp) << 4), kswap = (col & KX) << 4;
+  // transposing read: lane i of 16 points at row i / 2 of eight, 8 bytes of a piece, and receives column i of the piece
+  const int vrow = (lane & 15) >> 1;
+  const int vread = 32 * DP + (16 * (vrow >> 2) + 4 * grp + (vrow & 3)) * DP + ((vrow & KX) << 4) + 8 * (lane & 1);
   const float to_log2 = 1.44269504088896341f;
   const float cap = v.a.softcap;
   // scores in units of log 2: exp2 takes them as they are
@@ -284,7 +314,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
       continue;
     }
     const int64_t at = pos - before;  // inside the sequence
-    const int tile = (int)(at / sp.units);
+    const int tile = divide(at, sp.units);
     if (tile >= sp.tiles) {
       before += (int64_t)sp.tiles * sp.units;
       ++b;
@@ -301,6 +331,47 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
       u1 = sp.units;
     }
     pos += u1 - u0;
+
+    // page numbers are read a step before the loads that need them
+    const int* table = c.table + (int64_t)b * c.width;
+    const int last = max(sp.hi - 1, 0);
+    auto name = [&](int j0, int (&page)[2]) KV_CACHE_INLINE {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) page[h] = const_int(table, min(j0 + 16 * h, last) >> c.page_log2);
+    };
+    // 16 positions that no row sees, or that have no page, become zeros (an empty buffer); returns what is there
+    auto load = [&](int j0, const int (&pages)[2], int slot) KV_CACHE_INLINE {
+      uint8_t* const to = mine + slot * SLOT;
+      int there = 0;
+      int64_t scale_at[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = j0 + 16 * h, named = __builtin_amdgcn_readfirstlane(pages[h]);
+        const bool has = (unsigned)named < (unsigned)c.pages && j < sp.hi && j + 16 > sp.lo;
+        const int page = has ? named : 0, row = j & in_page;
+        there |= has ? 1 << h : 0;
+        const int64_t at = kv_row(c, page, head, row);
+        scale_at[h] = kv_scale(c, page, head, 0) * 4;
+        const __amdgpu_buffer_rsrc_t kr = kv_rsrc(c.codes[0] + at, has ? 16 * stride : 0);
+        const __amdgpu_buffer_rsrc_t vr = kv_rsrc(c.codes[1] + at, has ? 16 * stride : 0);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          load16_to_lds(kr, to + 16 * DP * h + 1024 * i, kfrom[i]);
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+          load16_to_lds(vr, to + 32 * DP + 16 * DP * h + 1024 * i, vfrom[h][i]);
+      }
+      // lanes 0 to 31: key scales of the 32 positions, 32 to 63: value scales
+      const int row = ((j0 & in_page) + (lane & 31)) & in_page;  // (the second 16 may begin a page)
+      const char* from = reinterpret_cast<const char*>(lane & 32 ? c.scales[1] : c.scales[0]) + (lane & 16 ? scale_at[1] : scale_at[0]);
+      load4_to_lds(from + (row >> c.block_log2) * 4, to + 64 * DP);
+      return there;
+    };
+    const int j_end = (sp.first + u1) * kUnit;
+    int j = (sp.first + u0) * kUnit + 32 * wave;
+    int there[DEPTH], pages[2];
+    const bool any = sp.hi > 0;
+    if (any) name(j, pages);
 
     // the tile's rows: packed row r is row r / group and head r % group
     const int r0 = tile * RT, rows = min(sp.s.n * v.a.group - r0, RT);
@@ -324,6 +395,22 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
     if (v.a.causal) all_hi = min(all_hi, sp.s.len - sp.s.n + r0 / v.a.group + 1);
     if (v.a.window > 0) all_lo = max(0, sp.s.len - sp.s.n + (r0 + rows - 1) / v.a.group - v.a.window + 1);
 
+    // q is here before the loop's loads are counted
+#pragma unroll
+    for (int t = 0; t < QT; ++t)
+#pragma unroll
+      for (int s = 0; s < DP / 32; ++s) asm volatile("" ::"v"(q[t][s]));
+    if (any) {
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        there[d] = 0;
+        if (j + d * kUnit < j_end) {
+          there[d] = load(j + d * kUnit, pages, d);
+          name(j + (d + 1) * kUnit, pages);
+        }
+      }
+    }
+
     floatx4 acc[QT][VT];
     float top[QT], sum[QT];
 #pragma unroll
@@ -334,84 +421,63 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
       for (int i = 0; i < VT; ++i) acc[t][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int* table = c.table + (int64_t)b * c.width;
-    // page numbers are read a step before the loads that need them
-    const int last = max(sp.hi - 1, 0);
-    auto name = [&](int j0, int (&page)[2]) {
+    auto step = [&](int slot) KV_CACHE_INLINE {
+      // this slot's loads are the oldest under way
+      if (j + (DEPTH - 1) * kUnit < j_end) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * PER) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const uint8_t* const from = mine + slot * SLOT;
+      uintx4 k[2][NI];
+      intx2 raw[VT];
+      float ks[2][S], vs[2][S];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) page[h] = table[min(j0 + 16 * h, last) >> c.page_log2];
-    };
-    // 16 positions that no row sees, or that have no page, are read from page 0 and masked
-    auto load = [&](int j0, const int (&pages)[2], DecodeLoads<DP, SMALL>& x) {
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int j = j0 + 16 * h, named = __builtin_amdgcn_readfirstlane(pages[h]);
-        x.there[h] = (unsigned)named < (unsigned)c.pages && j < sp.hi && j + 16 > sp.lo;
-        const int page = x.there[h] ? named : 0, row = j & in_page;
-        const int64_t at = kv_row(c, page, head, row);
-        const uint8_t* kp = c.codes[0] + at;
-        const uint8_t* vp = c.codes[1] + at;
+        for (int i = 0; i < NI; ++i) k[h][i] = *reinterpret_cast<const uintx4*>(from + 16 * DP * h + ((kread + 16 * i) ^ kswap));
 #pragma unroll
-        for (int s = 0; s < KW; ++s) x.k[h][s] = *reinterpret_cast<const uintx4*>(kp + koff[s]);
+      for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint8_t* p = vp + voff[i];
-          if constexpr (DP == 64) {
-            x.v[4 * h + i][0] = *reinterpret_cast<const uint32_t*>(p);
-          } else if constexpr (DP == 128) {
-            const uintx2 w = *reinterpret_cast<const uintx2*>(p);
-            x.v[4 * h + i][0] = w[0];
-            x.v[4 * h + i][1] = w[1];
-          } else {
-            const uintx4 w = *reinterpret_cast<const uintx4*>(p);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x.v[4 * h + i][e] = w[e];
-          }
+        for (int i = 0; i < S; ++i) {
+          ks[h][i] = *reinterpret_cast<const float*>(from + 64 * DP + 4 * (16 * h + 4 * grp + i));
+          vs[h][i] = *reinterpret_cast<const float*>(from + 64 * DP + 4 * (32 + 16 * h + 4 * grp + i));
         }
-        const int64_t sc = kv_scale(c, page, head, 0);
 #pragma unroll
-        for (int i = 0; i < DecodeLoads<DP, SMALL>::S; ++i) {
-          const int o = (row + 4 * grp + i) >> c.block_log2;
-          x.ks[h][i] = c.scales[0][sc + o];
-          x.vs[h][i] = c.scales[1][sc + o];
-        }
+      for (int t = 0; t < VT; ++t) raw[t] = read_columns(from + (vread ^ (t << 4)));
+      const int here = there[slot], j0 = j;
+      // the slot is empty again
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (j + DEPTH * kUnit < j_end) {
+        there[slot] = load(j + DEPTH * kUnit, pages, slot);
+        name(j + (DEPTH + 1) * kUnit, pages);
       }
-    };
-    auto step = [&](int j0, DecodeLoads<DP, SMALL>& x) {
       __builtin_amdgcn_sched_barrier(0);
-      if (!x.there[0] && !x.there[1]) return;
-      const bool edge = j0 < all_lo || j0 + 32 > all_hi || !x.there[0] || !x.there[1];
-      if (F8 && (j0 < sp.lo || j0 + 32 > sp.hi || !x.there[0] || !x.there[1])) {
+      if (here == 0) return;
+      const bool edge = j0 < all_lo || j0 + 32 > all_hi || here != 3;
+      if (F8 && (j0 < sp.lo || j0 + 32 > sp.hi)) {
         KV_CACHE_RARE();
         // positions that nobody sees may hold NaN codes, which a weight of zero does not cancel
+        uint32_t keep[2] = {0u, 0u};
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int j = j0 + 16 * (e >> 2) + 4 * grp + (e & 3);
-          const bool keep = x.there[e >> 2] && j >= sp.lo && j < sp.hi;
-#pragma unroll
-          for (int w = 0; w < KW; ++w) x.v[e][w] = keep ? x.v[e][w] : 0u;
+          const int at = j0 + 16 * (e >> 2) + 4 * grp + (e & 3);
+          keep[e >> 2] |= at >= sp.lo && at < sp.hi ? 0xffu << (8 * (e & 3)) : 0u;
         }
+#pragma unroll
+        for (int t = 0; t < VT; ++t) raw[t] = intx2{(int)(raw[t][0] & keep[0]), (int)(raw[t][1] & keep[1])};
       }
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int i = 0; i < DecodeLoads<DP, SMALL>::S; ++i) keep_to_its_rows(x.ks[h][i], x.vs[h][i]);
+        for (int i = 0; i < S; ++i) keep_to_its_rows(ks[h][i], vs[h][i]);
       floatx4 s[QT][2];
 #pragma unroll
       for (int t = 0; t < QT; ++t)
 #pragma unroll
         for (int h = 0; h < 2; ++h) s[t][h] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int m = 0; m < DP / 32; ++m)
 #pragma unroll
-        for (int m = 0; m < DP / 32; ++m) {
-          uintx4 w;
-          const uint32_t a = x.k[h][m >> 1][2 * (m & 1)], bb = x.k[h][m >> 1][2 * (m & 1) + 1];
-          w[0] = widen2<F8, 0>(a);
-          w[1] = widen2<F8, 2>(a);
-          w[2] = widen2<F8, 0>(bb);
-          w[3] = widen2<F8, 2>(bb);
-          const bf16x8 kk = __builtin_bit_cast(bf16x8, w);
+        for (int h = 0; h < 2; ++h) {
+          const bf16x8 kk = widen8<F8>(k[h][m >> 1][2 * (m & 1)], k[h][m >> 1][2 * (m & 1) + 1]);
 #pragma unroll
           for (int t = 0; t < QT; ++t) s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kk, q[t][m], s[t][h], 0, 0, 0);
           // one piece widened while the one before is multiplied, and no more of them in registers
@@ -422,10 +488,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
       for (int t = 0; t < QT; ++t) {
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int h = e >> 2, i = SMALL ? (e & 3) : 0;
-          y[e] = s[t][h][e & 3] * (x.ks[h][i] * factor);
-        }
+        for (int e = 0; e < 8; ++e) y[e] = s[t][e >> 2][e & 3] * (ks[e >> 2][SMALL ? (e & 3) : 0] * factor);
         if (cap > 0.0f) {
           KV_CACHE_RARE();
           // cap * tanh(y / cap), in units of log 2
@@ -439,8 +502,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
           KV_CACHE_RARE();
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            const int j = j0 + 16 * (e >> 2) + 4 * grp + (e & 3);
-            y[e] = x.there[e >> 2] && j >= sees_lo[t] && j < sees_hi[t] ? y[e] : -INFINITY;
+            const int at = j0 + 16 * (e >> 2) + 4 * grp + (e & 3);
+            y[e] = ((here >> (e >> 2)) & 1) && at >= sees_lo[t] && at < sees_hi[t] ? y[e] : -INFINITY;
           }
         }
         float most = y[0];
@@ -463,49 +526,31 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
           const int h = e >> 2;
           const float p0 = __builtin_amdgcn_exp2f(y[e] - top[t]), p1 = __builtin_amdgcn_exp2f(y[e + 1] - top[t]);
           sum[t] += p0 + p1;
-          const float v0 = x.vs[h][SMALL ? (e & 3) : 0], v1 = x.vs[h][SMALL ? (e & 3) + 1 : 0];
-          w[e >> 1] = pack_bf16x2(p0 * v0, p1 * v1);
+          w[e >> 1] = pack_bf16x2(p0 * vs[h][SMALL ? (e & 3) : 0], p1 * vs[h][SMALL ? (e & 3) + 1 : 0]);
         }
         p[t] = __builtin_bit_cast(bf16x8, w);
       }
-      static_for<0, VT / 2>([&](auto i) {
-        constexpr int I = 2 * decltype(i)::value;
-        bf16x8 va, vb;
-        columns<F8, I>(x.v, va, vb);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) {
-          acc[t][I] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(va, p[t], acc[t][I], 0, 0, 0);
-          acc[t][I + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vb, p[t], acc[t][I + 1], 0, 0, 0);
-        }
+      for (int i = 0; i < VT; ++i) {
+        const bf16x8 vv = widen8<F8>(raw[i][0], raw[i][1]);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[t], acc[t][i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-      });
+      }
     };
-
-    // two sets of loads take turns: the next 32 positions are under way while these are worked on
-    const int j_end = (sp.first + u1) * kUnit;
-    int j = (sp.first + u0) * kUnit + 32 * wave;
-    // (past the end of the range the loads name its last positions again: no load depends on a branch, so
-    // none of its uses is drawn up to it)
-    if (sp.hi > 0 && j < j_end) {
-      DecodeLoads<DP, SMALL> x0, x1;
-      int pages[2];
-      const int j_last = j_end - kUnit + 32 * wave;
-      name(j, pages);
-      load(j, pages, x0);
-      name(min(j + kUnit, j_last), pages);
-      while (true) {
-        load(min(j + kUnit, j_last), pages, x1);
-        name(min(j + 2 * kUnit, j_last), pages);
-        step(j, x0);
-        if ((j += kUnit) >= j_end) break;
-        load(min(j + kUnit, j_last), pages, x0);
-        name(min(j + 2 * kUnit, j_last), pages);
-        step(j, x1);
-        if ((j += kUnit) >= j_end) break;
+    if (any) {
+      while (j < j_end) {
+        static_for<0, DEPTH>([&](auto d) KV_CACHE_INLINE {
+          if (j < j_end) {
+            step(decltype(d)::value);
+            j += kUnit;
+          }
+        });
       }
     }
 
-    // the four waves' sums, 16 rows at a time
+    // the four waves' sums, 16 rows at a time, where the ring was (each wave has taken all it asked for)
+    float* const sums = reinterpret_cast<float*>(ring);
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       sum[t] += __shfl_xor(sum[t], 16);
@@ -526,12 +571,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
         const float m = __builtin_fmaxf(__builtin_fmaxf(tops[0][r], tops[1][r]), __builtin_fmaxf(tops[2][r], tops[3][r]));
         const float scale = __builtin_amdgcn_exp2f(top[t] - m);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float* o = &sums[wave][col * NF + (4 * grp + i) * VT];
-#pragma unroll
-          for (int n = 0; n < VT; n += 4)
-            *reinterpret_cast<floatx4*>(o + n) = floatx4{acc[t][n][i], acc[t][n + 1][i], acc[t][n + 2][i], acc[t][n + 3][i]} * scale;
-        }
+        for (int i = 0; i < VT; ++i)
+          *reinterpret_cast<floatx4*>(&sums[(wave * 16 + col) * NF + 16 * i + 4 * grp]) = acc[t][i] * scale;
       }
       __syncthreads();
       const int r = 16 * t + (tid >> 4);
@@ -546,7 +587,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
         for (int d = (tid & 15) * 4; d < c.head; d += 64) {
           floatx4 o = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int w = 0; w < 4; ++w) o += *reinterpret_cast<const floatx4*>(&sums[w][(tid >> 4) * NF + d]);
+          for (int w = 0; w < 4; ++w) o += *reinterpret_cast<const floatx4*>(&sums[(w * 16 + (tid >> 4)) * NF + d]);
           if (whole) {
             const uintx2 packed = {pack_bf16x2(o[0] * inverse, o[1] * inverse), pack_bf16x2(o[2] * inverse, o[3] * inverse)};
             *reinterpret_cast<uintx2*>(v.a.out + at_row * c.head + d) = packed;
@@ -564,7 +605,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_dec
         }
       }
     }
-    __syncthreads();  // tops and sums are the next range's
+    __syncthreads();  // tops, sums and the ring are the next range's
   }
 }
 
@@ -721,7 +762,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   const int kpos = lane / (DP / 16), kpiece = lane % (DP / 16);  // 64 / (DP / 16) positions at once
   const int vquad = lane % (DP < 128 ? DP / 4 : 32), vhalf = DP < 128 ? (lane / (DP / 4)) & 1 : h;
   auto page_of = [&](int u) {
-    return table[min(u * kStage + 16 * wave, hi - 1) >> c.page_log2];
+    return const_int(table, min(u * kStage + 16 * wave, hi - 1) >> c.page_log2);
   };
   auto fetch = [&](int u, int page) {
     const int j = u * kStage + 16 * wave;
@@ -948,7 +989,7 @@ DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_h
   const int64_t most = batch * (kFewRows / (16 * d.qt));
   if (few && d.tiles > most) d.tiles = most;
   const int64_t units = d.tiles * ((positions + kUnit - 1) / kUnit);
-  const int64_t slots = 512;
+  const int64_t slots = 256 * decode_residents(d.dp);
   int64_t w = (slots + kv_heads - 1) / kv_heads;
   if (w > units) w = units;
   d.workers = w < 1 ? 1 : (int)w;
