@@ -1,12 +1,11 @@
 // Book-keeping of a page pool on the device, and copying of whole pages.
 //
-// Book-keeping takes two launches.  The first ranks: its workgroup 0 decides the requests of
-// RESERVE, FORK and FREE (for the first two it collects as many free pages, lowest first, as they ask for)
-// while the others copy the reference counts; for COMPACT every workgroup ranks its own pages.  The
+// RESERVE, FORK and FREE take two launches.  Workgroup 0 of the first decides the requests (for the first two it
+// collects as many free pages, lowest first, as they ask for) while the others copy the reference counts.  The
 // second has one workgroup for each sequence, which writes its row of the new table and adjusts the counts
-// of its pages with integer atomics, whose order changes nothing.
+// of its pages with integer atomics, whose order changes nothing.  COMPACT takes three: count, rank, rewrite.
 //
-// Bound: the latency of two launches; the state is a few hundred kilobytes.
+// Bound: the latency of the launches; the state is a few hundred kilobytes.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -27,11 +26,12 @@ struct PagesView {
   int* status;
   // scratch
   int* slot;   // [pages] the free pages that are given away, in order
-  int* rank;   // [pages] COMPACT: a page's place among the free pages below U, or among the pages that move
-  int* mover;  // [pages] COMPACT: the pages that move, in order
+  int* rank;   // [pages] COMPACT: a page's place among the free pages below U, or among those that move
+  int* mover;  // [pages] COMPACT: the pages that move, the last one first
+  int* used;   // [pages / kRankPages] COMPACT: pages in use of each group
   int* plan;   // [batch] RESERVE: where the sequence's slots begin, or -1; FORK: its pair + 1; FREE: 1 if freed
   int* pair;   // [requests] FORK: the pair's slot, -1: granted without one, -2: refused
-  int* total;  // [1] COMPACT: pages in use
+  int* total;  // [2] COMPACT: pages in use, pages that move
   int batch, width, pages, page, requests;
 };
 
@@ -227,47 +227,65 @@ __global__ __launch_bounds__(256) void kv_pages_rows_kernel(PagesView v) {
   if (OP != XLA_AMD_KV_PAGES_RESERVE && threadIdx.x == 0) v.lens_out[b] = freed ? 0 : new_len;
 }
 
-// COMPACT, first launch: every workgroup counts the pages in use before its own and in all, then gives its
-// free pages below U and its pages in use from U on their ranks.
+constexpr int kRankPages = 4 * kThreads;  // pages of a ranking workgroup, four neighbours a thread
+
+__device__ __forceinline__ int4 four_counts(const PagesView& v, int64_t p) {
+  int4 r = {0, 0, 0, 0};
+  if (p + 3 < v.pages && ((uintptr_t)v.refs & 15) == 0) return *reinterpret_cast<const int4*>(v.refs + p);
+  if (p < v.pages) r.x = v.refs[p];
+  if (p + 1 < v.pages) r.y = v.refs[p + 1];
+  if (p + 2 < v.pages) r.z = v.refs[p + 2];
+  if (p + 3 < v.pages) r.w = v.refs[p + 3];
+  return r;
+}
+
+// COMPACT, first launch: pages in use among each kRankPages.
+__global__ __launch_bounds__(kThreads) void kv_pages_count_kernel(PagesView v) {
+  const int4 r = four_counts(v, (int64_t)blockIdx.x * kRankPages + 4 * threadIdx.x);
+  int all;
+  block_prefix((r.x != 0) + (r.y != 0) + (r.z != 0) + (r.w != 0), &all);
+  if (threadIdx.x == 0) v.used[blockIdx.x] = all;
+}
+
+// COMPACT, second launch: with U pages in use, the free pages below U and the pages in use from U on get their
+// ranks; the latter count from the end, so that no rank needs the number of them.
 __global__ __launch_bounds__(kThreads) void kv_pages_rank_kernel(PagesView v) {
-  const int first = blockIdx.x * kThreads;
-  int before = 0, used = 0;
-  for (int p = threadIdx.x; p < v.pages; p += kThreads) {
-    const int u = v.refs[p] != 0 ? 1 : 0;
+  int before = 0, used = 0, mine;
+  for (int i = threadIdx.x; i < (int)gridDim.x; i += kThreads) {
+    const int u = v.used[i];
     used += u;
-    before += p < first ? u : 0;
+    before += i < (int)blockIdx.x ? u : 0;
   }
-  int all_used, all_before, in_mine;
+  int all_used, all_before;
   block_prefix(used, &all_used);
   block_prefix(before, &all_before);
-  const int p = first + threadIdx.x;
-  const bool in = p < v.pages;
-  const bool mine = in && v.refs[p] != 0;
-  const int used_before = all_before + block_prefix(mine ? 1 : 0, &in_mine);
-  if (in && !mine && p < all_used) {
-    v.rank[p] = p - used_before;
-    v.slot[p - used_before] = p;
-  }
-  // the pages below U hold U minus the number of movers, so a page's place among the movers follows from
-  // the free pages below U: counted here as the pages in use before it, less those below U
-  __shared__ int below;
-  int mine_below = 0;
-  for (int q = threadIdx.x; q < all_used; q += kThreads) mine_below += v.refs[q] != 0 ? 1 : 0;
-  int sum;
-  block_prefix(mine_below, &sum);
-  if (threadIdx.x == 0) below = sum;
-  __syncthreads();
-  if (mine && p >= all_used) {
-    v.rank[p] = used_before - below;
-    v.mover[used_before - below] = p;
+  const int64_t p0 = (int64_t)blockIdx.x * kRankPages + 4 * threadIdx.x;
+  const int4 r = four_counts(v, p0);
+  const int counts[4] = {r.x, r.y, r.z, r.w};
+  int at = all_before + block_prefix((r.x != 0) + (r.y != 0) + (r.z != 0) + (r.w != 0), &mine);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = (int)(p0 + i);
+    if (p >= v.pages) break;
+    if (p == all_used) v.total[1] = all_used - at;  // pages that move: those in use, less those below U
+    if (counts[i] != 0) {
+      if (p >= all_used) {
+        v.rank[p] = all_used - 1 - at;
+        v.mover[all_used - 1 - at] = p;
+      }
+      ++at;
+    } else if (p < all_used) {
+      v.rank[p] = p - at;
+      v.slot[p - at] = p;
+    }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     v.total[0] = all_used;
-    v.total[1] = all_used - below;  // pages that move
+    if (all_used == v.pages) v.total[1] = 0;
   }
 }
 
-// COMPACT, second launch: the first `batch` workgroups rewrite the table, the others the counts and moves.
+// COMPACT, third launch: the first `batch` workgroups rewrite the table, the others the counts and moves.
 __global__ __launch_bounds__(256) void kv_pages_compact_kernel(PagesView v) {
   const int used = v.total[0], moving = v.total[1];
   if ((int)blockIdx.x < v.batch) {
@@ -275,7 +293,7 @@ __global__ __launch_bounds__(256) void kv_pages_compact_kernel(PagesView v) {
     const int len = v.lens[b], have = held_pages(v, len);
     for (int j = threadIdx.x; j < v.width; j += blockDim.x) {
       int page = j < have ? v.table[(int64_t)b * v.width + j] : -1;
-      if ((unsigned)page < (unsigned)v.pages && page >= used && v.refs[page] != 0) page = v.slot[v.rank[page]];
+      if ((unsigned)page < (unsigned)v.pages && page >= used && v.refs[page] != 0) page = v.slot[moving - 1 - v.rank[page]];
       v.table_out[(int64_t)b * v.width + j] = page;
     }
     if (threadIdx.x == 0) v.lens_out[b] = len;
@@ -286,11 +304,11 @@ __global__ __launch_bounds__(256) void kv_pages_compact_kernel(PagesView v) {
   int count = 0;
   if (p < used) {
     count = v.refs[p];
-    if (count == 0 && v.rank[p] < moving) count = v.refs[v.mover[v.rank[p]]];
+    if (count == 0) count = v.refs[v.mover[moving - 1 - v.rank[p]]];  // as many free pages below U as pages move
   }
   v.refs_out[p] = count;
   if (p < v.pages / 2) {
-    v.moves[2 * p] = p < moving ? v.mover[p] : -1;
+    v.moves[2 * p] = p < moving ? v.mover[moving - 1 - p] : -1;
     v.moves[2 * p + 1] = p < moving ? v.slot[p] : -1;
   }
 }
@@ -299,41 +317,66 @@ size_t Align16(size_t x) { return (x + 15) & ~(size_t)15; }
 
 struct CopyView {
   const int* moves;
-  int64_t num_moves;
-  int pages, buffers;
+  int pages, buffers, parts;  // parts: of the large buffers together
   uint8_t* base[XLA_AMD_KV_CACHE_MAX_BUFFERS];
   int64_t bytes[XLA_AMD_KV_CACHE_MAX_BUFFERS];
 };
 
-template <class T>
-__device__ __forceinline__ void copy_part(uint8_t* dst, const uint8_t* src, int64_t from, int64_t to) {
+// A workgroup copies kCopyPart bytes of one page of a large buffer, each thread four loads and then four stores
+// (one in flight a thread left 4.8 of the 6.5 TB/s that a plain copy reaches), or the pages of all small buffers.
+constexpr int kCopyPart = 16384, kCopySmall = 4096;
+
+template <class T, int N>
+__device__ __forceinline__ void copy_part(uint8_t* dst, const uint8_t* src, int64_t bytes, int first, int step) {
   T* d = reinterpret_cast<T*>(dst);
   const T* s = reinterpret_cast<const T*>(src);
-  for (int64_t i = from / sizeof(T) + threadIdx.x; i < to / (int64_t)sizeof(T); i += blockDim.x) d[i] = s[i];
+  const int64_t n = bytes / (int64_t)sizeof(T);
+  for (int64_t i = first; i < n; i += (int64_t)N * step) {
+    T x[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (i + k * step < n) x[k] = s[i + k * step];
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if (i + k * step < n) d[i + k * step] = x[k];
+  }
 }
 
-constexpr int64_t kCopyPart = 32768;  // bytes of a page that a workgroup copies
+__device__ __forceinline__ void copy_bytes(uint8_t* dst, const uint8_t* src, int64_t bytes, uint64_t low, int first, int step) {
+  if ((low & 15) == 0) copy_part<uintx4, 4>(dst, src, bytes, first, step);
+  else if ((low & 3) == 0) copy_part<uint32_t, 4>(dst, src, bytes, first, step);
+  else copy_part<uint8_t, 4>(dst, src, bytes, first, step);
+}
 
-// One workgroup for a part of one page of one buffer.
 __global__ __launch_bounds__(256) void kv_cache_copy_pages_kernel(CopyView v) {
-  const int64_t src = v.moves[2 * (int64_t)blockIdx.x], dst = v.moves[2 * (int64_t)blockIdx.x + 1];
+  const int move = blockIdx.x / (v.parts + 1), part = blockIdx.x % (v.parts + 1);
+  const int64_t src = const_int(v.moves, 2 * (int64_t)move), dst = const_int(v.moves, 2 * (int64_t)move + 1);
   if ((uint64_t)src >= (uint64_t)v.pages || (uint64_t)dst >= (uint64_t)v.pages || src == dst) return;
-  const int64_t bytes = v.bytes[blockIdx.z];
-  const int64_t from = blockIdx.y * kCopyPart, to = min(from + kCopyPart, bytes);
-  if (from >= bytes) return;
-  uint8_t* d = v.base[blockIdx.z] + dst * bytes;
-  const uint8_t* s = v.base[blockIdx.z] + src * bytes;
-  const uint64_t low = (uint64_t)(uintptr_t)v.base[blockIdx.z] | (uint64_t)bytes;
-  if ((low & 15) == 0) copy_part<uintx4>(d, s, from, to);
-  else if ((low & 3) == 0) copy_part<uint32_t>(d, s, from, to);
-  else copy_part<uint8_t>(d, s, from, to);
+  if (part == v.parts) {
+    // the small buffers, a wave each
+    for (int i = threadIdx.x >> 6; i < v.buffers; i += 4)
+      if (v.bytes[i] <= kCopySmall)
+        copy_bytes(v.base[i] + dst * v.bytes[i], v.base[i] + src * v.bytes[i], v.bytes[i],
+                   (uint64_t)(uintptr_t)v.base[i] | (uint64_t)v.bytes[i], threadIdx.x & 63, 64);
+    return;
+  }
+  int buffer = 0, at = part;
+  for (; buffer < v.buffers; ++buffer) {
+    const int n = v.bytes[buffer] <= kCopySmall ? 0 : (int)((v.bytes[buffer] + kCopyPart - 1) / kCopyPart);
+    if (at < n) break;
+    at -= n;
+  }
+  const int64_t bytes = v.bytes[buffer], from = (int64_t)at * kCopyPart;
+  copy_bytes(v.base[buffer] + dst * bytes + from, v.base[buffer] + src * bytes + from, min(bytes - from, (int64_t)kCopyPart),
+             (uint64_t)(uintptr_t)v.base[buffer] | (uint64_t)bytes, threadIdx.x, 256);
 }
 
 }  // namespace
 
 size_t KvCachePagesWorkspaceBytes(int64_t batch, int64_t pages, int64_t requests) {
   if (batch < 0 || pages < 0 || requests < 0) return 0;
-  return 3 * Align16((size_t)pages * 4) + Align16((size_t)batch * 4) + Align16((size_t)requests * 4) + 16;
+  return 3 * Align16((size_t)pages * 4) + Align16((size_t)batch * 4) + Align16((size_t)requests * 4) +
+         Align16(((size_t)pages / kRankPages + 1) * 4) + 16;
 }
 
 int LaunchKvCachePages(const XlaAmdKvCachePages& p, hipStream_t stream) {
@@ -384,7 +427,8 @@ int LaunchKvCachePages(const XlaAmdKvCachePages& p, hipStream_t stream) {
   v.mover = (int*)(w + 2 * page_ints);
   v.plan = (int*)(w + 3 * page_ints);
   v.pair = (int*)(w + 3 * page_ints + Align16((size_t)p.batch * 4));
-  v.total = (int*)(w + 3 * page_ints + Align16((size_t)p.batch * 4) + Align16((size_t)p.requests * 4));
+  v.used = (int*)((char*)v.pair + Align16((size_t)p.requests * 4));
+  v.total = (int*)((char*)v.used + Align16(((size_t)p.pages / kRankPages + 1) * 4));
   v.batch = (int)p.batch;
   v.width = (int)p.table_width;
   v.pages = (int)p.pages;
@@ -410,8 +454,9 @@ int LaunchKvCachePages(const XlaAmdKvCachePages& p, hipStream_t stream) {
       break;
     default: {
       SetLastKernel("kv_cache_pages_compact");
-      const int ranks = (int)((p.pages + kThreads - 1) / kThreads);
-      kv_pages_rank_kernel<<<ranks > 0 ? ranks : 1, kThreads, 0, stream>>>(v);
+      const int ranks = (int)(p.pages / kRankPages) + 1;
+      kv_pages_count_kernel<<<ranks, kThreads, 0, stream>>>(v);
+      kv_pages_rank_kernel<<<ranks, kThreads, 0, stream>>>(v);
       const int64_t grid = p.batch + (p.pages + 255) / 256;
       if (grid > 0) kv_pages_compact_kernel<<<(unsigned)grid, 256, 0, stream>>>(v);
     }
@@ -428,22 +473,24 @@ int LaunchKvCacheCopyPages(const XlaAmdKvCacheCopyPages& p, hipStream_t stream) 
   if (p.num_moves > 0 && (!p.moves || ((uintptr_t)p.moves & 3))) return Fail(kBad, "kv_cache_copy_pages: null or unaligned moves");
   CopyView v{};
   v.moves = p.moves;
-  v.num_moves = p.num_moves;
   v.pages = (int)p.pages;
   v.buffers = (int)p.num_buffers;
-  int64_t most = 0;
+  int64_t most = 0, parts = 0;
   for (int i = 0; i < v.buffers; ++i) {
-    if (p.page_bytes[i] < 0 || p.page_bytes[i] > (int64_t)kCopyPart * 65535)
-      return Fail(kBad, "kv_cache_copy_pages: a page of a buffer holds at most %lld bytes", (long long)kCopyPart * 65535);
+    if (p.page_bytes[i] < 0 || p.page_bytes[i] > INT32_MAX)
+      return Fail(kBad, "kv_cache_copy_pages: a page of a buffer holds at most 2^31 - 1 bytes");
     if (!p.buffers[i] && p.pages > 0 && p.page_bytes[i] > 0) return Fail(kBad, "kv_cache_copy_pages: null buffer");
     v.base[i] = (uint8_t*)p.buffers[i];
     v.bytes[i] = p.page_bytes[i];
     if (v.bytes[i] > most) most = v.bytes[i];
+    if (v.bytes[i] > kCopySmall) parts += (v.bytes[i] + kCopyPart - 1) / kCopyPart;
   }
   if (p.num_moves == 0 || p.pages == 0 || most == 0) return 0;
+  if ((parts + 1) * p.num_moves > INT32_MAX)
+    return Fail(kBad, "kv_cache_copy_pages: at most 2^31 - 1 moves times parts of %d bytes", kCopyPart);
+  v.parts = (int)parts;
   SetLastKernel("kv_cache_copy_pages");
-  const dim3 grid((unsigned)p.num_moves, (unsigned)((most + kCopyPart - 1) / kCopyPart), (unsigned)v.buffers);
-  kv_cache_copy_pages_kernel<<<grid, 256, 0, stream>>>(v);
+  kv_cache_copy_pages_kernel<<<(unsigned)((parts + 1) * p.num_moves), 256, 0, stream>>>(v);
   return CheckLaunch("kv_cache_copy_pages");
 }
 

@@ -101,49 +101,26 @@ __device__ __forceinline__ int touched_blocks(const KvCacheView& c, int b) {
   return ((s.len - 1) >> c.block_log2) - (max(s.len - s.n, 0) >> c.block_log2) + 1;
 }
 
-// One wave for a block of one head of k or v: the block's new rows are read twice (the second time from L2),
-// eight values a lane.
-template <bool F8>
-__global__ __launch_bounds__(256) void kv_cache_write_kernel(KvCacheView c, const uint16_t* __restrict__ k,
-                                                             const uint16_t* __restrict__ v) {
-  const int lane = threadIdx.x & 63;
-  const int hv = blockIdx.y * 4 + (threadIdx.x >> 6);
-  if (hv >= 2 * c.heads) return;
-  const int which = hv >= c.heads ? 1 : 0, head = hv - which * c.heads;
-  int64_t index;
-  const int b = kv_find_item(c.batch, blockIdx.x, lane, &index, [&](int s) { return touched_blocks(c, s); });
-  if (b < 0) return;
-  const KvSequence s = kv_sequence(c, b);
-  const int start = max(s.len - s.n, 0);
-  const int first = ((start >> c.block_log2) + (int)index) << c.block_log2;  // the block's first position
-  const int from = max(first, start), to = min(first + (1 << c.block_log2), s.len);
-  const int page = kv_page(c, b, first);
-  if (page < 0) return;
-  const int in_page = first & ((1 << c.page_log2) - 1);
-  const uint16_t* x = (which ? v : k) + ((int64_t)(s.row0 + s.n - (s.len - from)) * c.heads + head) * c.head;
-  uint8_t* codes = c.codes[which] + kv_row(c, page, head, in_page);
-  float* scale_at = c.scales[which] + kv_scale(c, page, head, in_page);
+// Eight bf16 of a row, and their largest magnitude as bits: every NaN is above every number.
+__device__ __forceinline__ uint32_t largest(uintx4 w) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7fff0000u, w[i] & 0x7fff0000u));
+  return top;
+}
 
-  const int chunks = c.head >> 3;  // of eight values
-  const int units = (to - from) * chunks;
-  uint32_t top = 0;  // the largest |x|, as bits: every NaN is above every number
-  for (int u = lane; u < units; u += 64) {
-    const int r = u / chunks, at = (u - r * chunks) * 8;
-    const uintx4 w = *reinterpret_cast<const uintx4*>(x + (int64_t)r * c.heads * c.head + at);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7fff0000u, w[i] & 0x7fff0000u));
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, off));
-  const float amax = bits_to_f32(top);
-  float scale = (amax == amax ? amax : bits_to_f32(0x7fc00000u)) / (F8 ? 448.0f : 127.0f);
-  const int held = from - first;  // rows of the sequence that the block held before
-  if (held > 0) {
+// Re-scales the codes that a block held before (its first `units` groups of eight) where its scale grows;
+// returns the block's scale.
+template <bool F8>
+__device__ __forceinline__ float settle_scale(uint32_t top, int units, int lane, float* scale_at, uint8_t* codes) {
+  const float amax = bits_to_f32(top > 0x7f800000u ? 0x7fc00000u : top);
+  float scale = amax / (F8 ? 448.0f : 127.0f);
+  if (units > 0) {
     const float old = *scale_at;
     if (old > scale || old != old) scale = old;
     if (scale != old) {
       const float ratio = old / scale;
-      for (int u = lane; u < held * chunks; u += 64) {
+      for (int u = lane; u < units; u += 64) {
         uintx2* at = reinterpret_cast<uintx2*>(codes) + u;
         const uintx2 w = *at;
         uintx2 o;
@@ -158,27 +135,90 @@ __global__ __launch_bounds__(256) void kv_cache_write_kernel(KvCacheView c, cons
       }
     }
   }
-  const bool some = scale > 0.0f;  // a zero or NaN scale: all codes 0
-  const bool fast = ordinary_divisor(scale);
-  const float inverse = 1.0f / scale;
-  for (int u = lane; u < units; u += 64) {
-    const int r = u / chunks, at = (u - r * chunks) * 8;
-    const uintx4 w = *reinterpret_cast<const uintx4*>(x + (int64_t)r * c.heads * c.head + at);
-    float t[8];
+  return scale;
+}
+
+template <bool F8>
+__device__ __forceinline__ uintx2 quantise8(uintx4 w, float scale, float inverse, bool fast) {
+  float t[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      t[2 * i] = bf16lo_to_f32(w[i]);
-      t[2 * i + 1] = bf16hi_to_f32(w[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float q = fast ? div_by_ordinary(t[i], scale, inverse) : t[i] / scale;
-      t[i] = some ? q : 0.0f;
-    }
-    uintx2 o = {to_codes<F8>(t), to_codes<F8>(t + 4)};
-    *reinterpret_cast<uintx2*>(codes + (int64_t)(held + r) * c.head + at) = o;
+  for (int i = 0; i < 4; ++i) {
+    t[2 * i] = bf16lo_to_f32(w[i]);
+    t[2 * i + 1] = bf16hi_to_f32(w[i]);
   }
-  if (lane == 0) *scale_at = scale;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float q = fast ? div_by_ordinary(t[i], scale, inverse) : t[i] / scale;
+    t[i] = scale > 0.0f ? q : 0.0f;  // a zero or NaN scale: all codes 0
+  }
+  return uintx2{to_codes<F8>(t), to_codes<F8>(t + 4)};
+}
+
+// One wave for a block and head, keys and values together: finding the block and its page costs a wave more than
+// its arithmetic does.  A lane holds HELD groups of eight values of each while the maximum is found (16 rows of 128
+// values, or one row of a decode step); a block with more new values reads them again, from L2.
+// 8192 sequences' worth of waves fit the device: 16 prompts of 16352 rows over 8 heads of 128, 16-row blocks, take
+// two rounds of waves less than with a wave for keys and one for values that read twice.
+constexpr int kHeld = 4;
+
+template <bool F8>
+__global__ __launch_bounds__(256) void kv_cache_write_kernel(KvCacheView c, const uint16_t* __restrict__ k,
+                                                             const uint16_t* __restrict__ v) {
+  const int lane = threadIdx.x & 63;
+  const int head = blockIdx.y * 4 + (threadIdx.x >> 6);
+  if (head >= c.heads) return;
+  int64_t index;
+  const int b = kv_find_item(c.batch, blockIdx.x, lane, &index, [&](int s) { return touched_blocks(c, s); });
+  if (b < 0) return;
+  const KvSequence s = kv_sequence(c, b);
+  const int start = max(s.len - s.n, 0);
+  const int first = ((start >> c.block_log2) + (int)index) << c.block_log2;  // the block's first position
+  const int from = max(first, start), to = min(first + (1 << c.block_log2), s.len);
+  const int page = kv_page(c, b, first);
+  if (page < 0) return;
+  const int in_page = first & ((1 << c.page_log2) - 1);
+  const int chunks = c.head >> 3;  // groups of eight values in a row
+  const int held = from - first;   // rows of the sequence that the block held before
+  const int units = (to - from) * chunks;
+  const int64_t x = ((int64_t)(s.row0 + s.n - (s.len - from)) * c.heads + head) * c.head;
+  const int64_t row_stride = (int64_t)c.heads * c.head;
+  const int64_t code = kv_row(c, page, head, in_page), scale_at = kv_scale(c, page, head, in_page);
+  auto read = [&](const uint16_t* src, int u) {
+    const int r = u / chunks;
+    return *reinterpret_cast<const uintx4*>(src + x + r * row_stride + (u - r * chunks) * 8);
+  };
+  uintx4 held_values[2][kHeld];
+  uint32_t top[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i) {
+    const int u = lane + 64 * i;
+#pragma unroll
+    for (int w = 0; w < 2; ++w) held_values[w][i] = u < units ? read(w ? v : k, u) : uintx4{0u, 0u, 0u, 0u};
+  }
+#pragma unroll
+  for (int i = 0; i < kHeld; ++i)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) top[w] = max(top[w], largest(held_values[w][i]));
+  for (int u = lane + 64 * kHeld; u < units; u += 64)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) top[w] = max(top[w], largest(read(w ? v : k, u)));
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) top[w] = max(top[w], (uint32_t)__shfl_xor((int)top[w], off));
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    uint8_t* codes = c.codes[w] + code;
+    const float scale = settle_scale<F8>(top[w], held * chunks, lane, c.scales[w] + scale_at, codes);
+    const bool fast = ordinary_divisor(scale);
+    const float inverse = 1.0f / scale;
+    uintx2* out = reinterpret_cast<uintx2*>(codes + (int64_t)held * c.head);
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (lane + 64 * i < units) out[lane + 64 * i] = quantise8<F8>(held_values[w][i], scale, inverse, fast);
+    for (int u = lane + 64 * kHeld; u < units; u += 64) out[u] = quantise8<F8>(read(w ? v : k, u), scale, inverse, fast);
+    if (lane == 0) c.scales[w][scale_at] = scale;
+  }
 }
 
 }  // namespace
@@ -193,7 +233,7 @@ int LaunchKvCacheWrite(const XlaAmdKvCacheWrite& p, hipStream_t stream) {
   // n rows touch at most n blocks and at most (n - 2) / block + 2
   int64_t items = ((int64_t)c.rows >> c.block_log2) + 2 * (int64_t)c.batch;
   if (items > c.rows) items = c.rows;
-  const dim3 grid((unsigned)items, (unsigned)((2 * c.heads + 3) / 4));
+  const dim3 grid((unsigned)items, (unsigned)((c.heads + 3) / 4));
   if (p.cache.cache_dtype == XLA_FFI_DataType_F8E4M3FN) {
     SetLastKernel("kv_cache_write_f8");
     kv_cache_write_kernel<true><<<grid, 256, 0, stream>>>(c, (const uint16_t*)p.k, (const uint16_t*)p.v);

@@ -7,11 +7,14 @@ HIP stream.  torch only supplies device memory and the stream.  bf16 operands ar
 s8 weights ``int8``, s4 weights ``uint8`` holding two values per byte (low nibble first)
 with the logical shape passed separately.
 """
+import threading
+
 import torch
 
 from . import dtypes, ffi
 
 _host = None
+_running = threading.Lock()  # the host carries one stream: from setting it to the call's end no other thread sets it
 
 
 def host():
@@ -46,8 +49,9 @@ class Call:
         self.target, self.frame, self.result, self._keep = target, frame, result, keep
 
     def run(self):
-        self.frame.host.stream = _stream()
-        ffi.invoke(self.target, self.frame)
+        with _running:
+            self.frame.host.stream = _stream()
+            ffi.invoke(self.target, self.frame)
         return self.result
 
 
@@ -220,11 +224,23 @@ class _DeviceCall(Call):
 
     def __init__(self, device, *args, **kw):
         super().__init__(*args, **kw)
-        self._device = device
+        self._device = device.index
+        self._handler = getattr(ffi.library(), ffi.HANDLER_SYMBOLS[self.target])
+        self._address = self.frame.address()
 
     def run(self):
-        with torch.cuda.device(self._device):
-            return super().run()
+        if torch.cuda.current_device() != self._device:
+            with torch.cuda.device(self._device):
+                return self.run()
+        stream = torch._C._cuda_getCurrentRawStream(self._device)
+        host = self.frame.host
+        with _running:
+            if host.stream != stream:
+                host.stream = stream
+            error = self._handler(self._address)
+            if error:
+                raise ffi.FfiError(*host.take_error(error))
+        return self.result
 
 
 def _cache_operands(k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets):
