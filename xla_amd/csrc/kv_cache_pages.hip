@@ -335,10 +335,10 @@ __device__ __forceinline__ void copy_part(uint8_t* dst, const uint8_t* src, int6
     T x[N];
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      if (i + k * step < n) x[k] = s[i + k * step];
+      if (i + k * step < n) x[k] = __builtin_nontemporal_load(&s[i + k * step]);
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      if (i + k * step < n) d[i + k * step] = x[k];
+      if (i + k * step < n) __builtin_nontemporal_store(x[k], &d[i + k * step]);
   }
 }
 

@@ -101,12 +101,15 @@ __device__ __forceinline__ int touched_blocks(const KvCacheView& c, int b) {
   return ((s.len - 1) >> c.block_log2) - (max(s.len - s.n, 0) >> c.block_log2) + 1;
 }
 
-// Eight bf16 of a row, and their largest magnitude as bits: every NaN is above every number.
-__device__ __forceinline__ uint32_t largest(uintx4 w) {
-  uint32_t top = 0;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, max((w[i] << 16) & 0x7fff0000u, w[i] & 0x7fff0000u));
-  return top;
+typedef uint16_t ushortx2 __attribute__((ext_vector_type(2)));
+
+// The larger magnitudes of two pairs of bf16, as bits: every NaN is above every number.
+__device__ __forceinline__ uint32_t larger_pair(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(ushortx2, a), __builtin_bit_cast(ushortx2, b & 0x7fff7fffu)));
+}
+
+__device__ __forceinline__ uint32_t larger_pairs(uint32_t top, uintx4 w) {
+  return larger_pair(larger_pair(larger_pair(larger_pair(top, w[0]), w[1]), w[2]), w[3]);
 }
 
 // Re-scales the codes that a block held before (its first `units` groups of eight) where its scale grows;
@@ -138,18 +141,44 @@ __device__ __forceinline__ float settle_scale(uint32_t top, int units, int lane,
   return scale;
 }
 
+// Eight values over an ordinary scale that is at least their maximum / qmax: the quotients are numbers and none
+// rounds beyond qmax, so nothing is selected or clamped.  A zero quotient has lost its sign in div_by_ordinary's
+// correction; the codes take the values' signs (s8 has no negative zero).  s8: 1.5 * 2^23 + q holds the nearest
+// even integer in its low byte.
 template <bool F8>
-__device__ __forceinline__ uintx2 quantise8(uintx4 w, float scale, float inverse, bool fast) {
+__device__ __forceinline__ uintx2 quantise8_ordinary(uintx4 w, float scale, float inverse) {
   float t[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    t[2 * i] = bf16lo_to_f32(w[i]);
-    t[2 * i + 1] = bf16hi_to_f32(w[i]);
+  for (int i = 0; i < 8; ++i) {
+    const float x = i & 1 ? bf16hi_to_f32(w[i >> 1]) : bf16lo_to_f32(w[i >> 1]);
+    const float q = x * inverse;
+    t[i] = __builtin_fmaf(__builtin_fmaf(-q, scale, x), inverse, q);
+    if (!F8) t[i] += 12582912.0f;
   }
+  uintx2 o;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (F8) {
+      const uint32_t signs = __builtin_amdgcn_perm(w[2 * h + 1], w[2 * h], 0x07050301u);  // high bytes of the four values
+      const uint32_t codes = pack_f8x4(t[4 * h], t[4 * h + 1], t[4 * h + 2], t[4 * h + 3]);
+      o[h] = (codes & 0x7f7f7f7fu) | (signs & 0x80808080u);
+    } else {
+      const uint32_t lo = __builtin_amdgcn_perm(f32_to_bits(t[4 * h + 1]), f32_to_bits(t[4 * h]), 0x0c0c0400u);
+      const uint32_t hi = __builtin_amdgcn_perm(f32_to_bits(t[4 * h + 3]), f32_to_bits(t[4 * h + 2]), 0x04000c0cu);
+      o[h] = lo | hi;
+    }
+  }
+  return o;
+}
+
+// The same for any scale; a zero or NaN one gives code 0, as does a quotient that is no number.
+template <bool F8>
+__device__ __forceinline__ uintx2 quantise8(uintx4 w, float scale) {
+  float t[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float q = fast ? div_by_ordinary(t[i], scale, inverse) : t[i] / scale;
-    t[i] = scale > 0.0f ? q : 0.0f;  // a zero or NaN scale: all codes 0
+    const float x = i & 1 ? bf16hi_to_f32(w[i >> 1]) : bf16lo_to_f32(w[i >> 1]);
+    t[i] = scale > 0.0f ? x / scale : 0.0f;
   }
   return uintx2{to_codes<F8>(t), to_codes<F8>(t + 4)};
 }
@@ -198,25 +227,30 @@ __global__ __launch_bounds__(256) void kv_cache_write_kernel(KvCacheView c, cons
 #pragma unroll
   for (int i = 0; i < kHeld; ++i)
 #pragma unroll
-    for (int w = 0; w < 2; ++w) top[w] = max(top[w], largest(held_values[w][i]));
+    for (int w = 0; w < 2; ++w) top[w] = larger_pairs(top[w], held_values[w][i]);
   for (int u = lane + 64 * kHeld; u < units; u += 64)
 #pragma unroll
-    for (int w = 0; w < 2; ++w) top[w] = max(top[w], largest(read(w ? v : k, u)));
+    for (int w = 0; w < 2; ++w) top[w] = larger_pairs(top[w], read(w ? v : k, u));
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1)
 #pragma unroll
-    for (int w = 0; w < 2; ++w) top[w] = max(top[w], (uint32_t)__shfl_xor((int)top[w], off));
+    for (int w = 0; w < 2; ++w) top[w] = larger_pair(top[w], (uint32_t)__shfl_xor((int)top[w], off));
+#pragma unroll
+  for (int w = 0; w < 2; ++w) top[w] = max(top[w] << 16, top[w] & 0xffff0000u);
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
     uint8_t* codes = c.codes[w] + code;
     const float scale = settle_scale<F8>(top[w], held * chunks, lane, c.scales[w] + scale_at, codes);
-    const bool fast = ordinary_divisor(scale);
-    const float inverse = 1.0f / scale;
     uintx2* out = reinterpret_cast<uintx2*>(codes + (int64_t)held * c.head);
+    if (ordinary_divisor(scale)) {
+      const float inverse = 1.0f / scale;
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-      if (lane + 64 * i < units) out[lane + 64 * i] = quantise8<F8>(held_values[w][i], scale, inverse, fast);
-    for (int u = lane + 64 * kHeld; u < units; u += 64) out[u] = quantise8<F8>(read(w ? v : k, u), scale, inverse, fast);
+      for (int i = 0; i < kHeld; ++i)
+        if (lane + 64 * i < units) out[lane + 64 * i] = quantise8_ordinary<F8>(held_values[w][i], scale, inverse);
+      for (int u = lane + 64 * kHeld; u < units; u += 64) out[u] = quantise8_ordinary<F8>(read(w ? v : k, u), scale, inverse);
+    } else {
+      for (int u = lane; u < units; u += 64) out[u] = quantise8<F8>(read(w ? v : k, u), scale);
+    }
     if (lane == 0) c.scales[w][scale_at] = scale;
   }
 }
