@@ -23,6 +23,14 @@ struct AttentionView {
   int causal, window;
 };
 
+// A tile of packed rows whose positions several workgroups share.
+struct __attribute__((aligned(16))) CutTile {
+  int row0;    // the sequence's first row
+  int first;   // packed row of the sequence where the tile begins
+  int rows;    // 0: no tile
+  int pieces;
+};
+
 // ---- few rows for each sequence: the cache is streamed once ------------------------------------------
 //
 // A workgroup of four waves takes the packed rows (row, head of the group) of one sequence and cache head, 16
@@ -40,7 +48,8 @@ struct AttentionView {
 // Where the keys are split: all sequences' units (times their tiles of rows) stand in one line, which is cut
 // into as many equal pieces as there are workers for a head, so a batch of mixed lengths fills the device
 // evenly.  A range that covers a tile whole writes the result; any other writes f32 sums to the
-// scratch, at most two for each worker, and a second launch joins them in order.
+// scratch, at most two for each worker, and a second launch joins them in order.  The worker in whose range a cut
+// tile begins notes where its pieces are, so the second launch looks for nothing.
 //
 // Bound: HBM, 2 (head + 4 / block) bytes for each position and cache head.
 constexpr int kUnit = 128;
@@ -48,6 +57,7 @@ constexpr int kUnit = 128;
 struct DecodeView {
   AttentionView a;
   float* partial;   // [heads][2 * workers][tile rows][head + 2], or null: ranges are whole tiles
+  CutTile* cuts;    // [workers], of the tile that a worker begins and others go on with
   int workers;      // for each head
   int rows_from, rows_to;  // sequences with rows_from < n * group <= rows_to are this kernel's
 };
@@ -78,67 +88,48 @@ __device__ __forceinline__ int64_t shfl64(int64_t x, int src) {
   return (int64_t)((uint64_t)(uint32_t)hi << 32 | (uint32_t)lo);
 }
 
-// Where an entry of the line lies, whose entries are units (TILES false) or tiles of rows.
+// Where an entry of a line lies in which sequence b has entries(b) of them.
 struct LineSpot {
-  int b;               // the sequence, -1 past the end
-  int64_t before;      // entries before the sequence's
-  int64_t units_before, total_units;
+  int b;           // the sequence, -1 past the end
+  int64_t before;  // entries before the sequence's
+  int64_t total;
 };
 
-// 64 sequences at a time: lane l holds sequence b0 + l, scans over the lanes give what lies before each.  `at` is
-// asked for once the total is known.
-template <int RT, bool TILES, class At>
-__device__ LineSpot line_find(const DecodeView& v, int lane, At at) {
-  const int batch = v.a.c.batch;
-  LineSpot r{-1, 0, 0, 0};
-  auto cost = [&](int b, int64_t* tiles, int64_t* units) {
-    *tiles = *units = 0;
-    if (b < batch) {
-      const DecodeSpan s = decode_span<RT>(v, b);
-      *tiles = s.tiles;
-      *units = (int64_t)s.tiles * s.units;
-    }
-  };
-  auto scan = [&](int64_t x) {
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int64_t t = shfl64(x, lane - off);
-      if (lane >= off) x += t;
-    }
-    return x;
-  };
-  int64_t tiles, units;
-  cost(lane, &tiles, &units);
+// 64 sequences at a time: lane l holds sequence b0 + l, scans over the lanes give what lies before each.  Entry
+// at(total) is looked for.
+template <class Entries, class At>
+__device__ __forceinline__ LineSpot line_find(int batch, int lane, Entries entries, At at) {
+  LineSpot r{-1, 0, 0};
+  auto cost = [&](int b) -> int64_t { return b < batch ? entries(b) : 0; };
+  int64_t units = cost(lane);
   if (batch > 64) {
     int64_t sum = units;
-    for (int b = lane + 64; b < batch; b += 64) {
-      int64_t t, u;
-      cost(b, &t, &u);
-      sum += u;
-    }
+    for (int b = lane + 64; b < batch; b += 64) sum += cost(b);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) sum += shfl64(sum, lane ^ off);
-    r.total_units = uniform64(sum);
+    r.total = uniform64(sum);
   }
-  int64_t seen = 0, seen_units = 0, want = batch > 64 ? at(r.total_units) : 0;
+  int64_t seen = 0, want = batch > 64 ? at(r.total) : 0;
   for (int b0 = 0; b0 < batch; b0 += 64) {
-    if (b0 > 0) cost(b0 + lane, &tiles, &units);
-    const int64_t upto_units = scan(units);
-    if (batch <= 64) {
-      r.total_units = uniform64(shfl64(upto_units, 63));
-      want = at(r.total_units);
+    if (b0 > 0) units = cost(b0 + lane);
+    int64_t upto = units;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int64_t t = shfl64(upto, lane - off);
+      if (lane >= off) upto += t;
     }
-    const int64_t n = TILES ? tiles : units, upto = TILES ? scan(tiles) : upto_units;
-    const unsigned long long hit = __ballot(want < seen + upto && want >= seen + upto - n);
+    if (batch <= 64) {
+      r.total = uniform64(shfl64(upto, 63));
+      want = at(r.total);
+    }
+    const unsigned long long hit = __ballot(want < seen + upto && want >= seen + upto - units);
     if (hit != 0ull) {
       const int src = __builtin_ctzll(hit);
       r.b = __builtin_amdgcn_readfirstlane(b0 + src);
-      r.before = seen + uniform64(shfl64(upto - n, src));
-      r.units_before = seen_units + uniform64(shfl64(upto_units - units, src));
+      r.before = seen + uniform64(shfl64(upto - units, src));
       return r;
     }
     seen += uniform64(shfl64(upto, 63));
-    seen_units += uniform64(shfl64(upto_units, 63));
   }
   return r;
 }
@@ -275,13 +266,20 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
     return;
   }
   int64_t piece = 1;
-  const LineSpot spot = line_find<RT, false>(v, lane, [&](int64_t total) {
-    piece = worker_piece(total, v.workers);
-    return piece * blockIdx.x;
-  });
+  const LineSpot spot = line_find(
+      c.batch, lane,
+      [&](int b) {
+        const DecodeSpan s = decode_span<RT>(v, b);
+        return (int64_t)s.tiles * s.units;
+      },
+      [&](int64_t total) {
+        piece = worker_piece(total, v.workers);
+        return piece * blockIdx.x;
+      });
   int64_t pos = piece * blockIdx.x, before = spot.before;
-  const int64_t stop = min(pos + piece, spot.total_units);
+  const int64_t stop = min(pos + piece, spot.total);
   int b = spot.b;
+  CutTile cut = {0, 0, 0, 0};
 
   // Where a lane's 16 bytes of a load come from: LDS is filled in order, so the pieces of a row are exchanged at the
   // source.  Keys: piece ^ (row & 7), met again when 16 rows are read a piece at a time; values: piece ^ (row & 3, and
@@ -561,6 +559,8 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
       }
     }
     const bool whole = u0 == 0 && u1 == sp.units;
+    if (u0 == 0 && !whole)
+      cut = CutTile{sp.s.row0, r0, rows, divide(before + (int64_t)(tile + 1) * sp.units - 1, piece) - (int)blockIdx.x + 1};
     // a range that begins inside a tile is its worker's first, one that ends inside its last
     float* part = v.partial + ((int64_t)head * 2 * v.workers + 2 * blockIdx.x + (u0 == 0 ? 1 : 0)) * RT * (c.head + 2);
 #pragma unroll
@@ -607,64 +607,7 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
     }
     __syncthreads();  // tops, sums and the ring are the next range's
   }
-}
-
-// One row's result from the sums of `count` pieces, part(w) apart; a wave for a row.  The lanes first hold a piece's
-// maximum and sum each, then go along the head, all pieces' sums under way together.
-template <int RT, class Part>
-__device__ __forceinline__ void join_row(const AttentionView& v, const KvSequence& s, int r0, int r, int head, int lane, int count,
-                                         Part part) {
-  const int size = v.c.head;
-  float m = -1e30f;
-  for (int w = lane; w < count; w += 64) m = __builtin_fmaxf(m, part(w)[RT * size + r]);
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) m = __builtin_fmaxf(m, __shfl_xor(m, off));
-  float l = 0.0f;
-  floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int d = min(4 * lane, size - 4);
-  for (int w0 = 0; w0 < count; w0 += 64) {
-    const int here = min(count - w0, 64);
-    float scale = 0.0f;
-    if (lane < here) {
-      const float* p = part(w0 + lane) + RT * size + r;
-      scale = __builtin_amdgcn_exp2f(p[0] - m);
-      l += p[RT] * scale;
-    }
-#pragma unroll 4
-    for (int w = 0; w < here; ++w) o += *reinterpret_cast<const floatx4*>(part(w0 + w) + (int64_t)r * size + d) * __shfl(scale, w);
-  }
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off);
-  const int i = (r0 + r) / v.group, g = r0 + r - i * v.group;
-  const int64_t at_row = (int64_t)(s.row0 + i) * v.q_heads + head * v.group + g;
-  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
-  if (4 * lane < size)
-    *reinterpret_cast<uintx2*>(v.out + at_row * size + d) =
-        uintx2{pack_bf16x2(o[0] * inverse, o[1] * inverse), pack_bf16x2(o[2] * inverse, o[3] * inverse)};
-  if (lane == 0 && v.lse) v.lse[at_row] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.693147180559945309f;
-}
-
-// Joins the sums of the workers that share a tile, in their order; a workgroup for four rows of a tile and head.
-template <int RT>
-__global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(DecodeView v) {
-  const KvCacheView& c = v.a.c;
-  const int lane = threadIdx.x & 63, head = blockIdx.y, at = blockIdx.x / (RT / 4);
-  const int r = (blockIdx.x % (RT / 4)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const LineSpot spot = line_find<RT, true>(v, lane, [&](int64_t) { return (int64_t)at; });
-  if (spot.b < 0) return;
-  const int64_t piece = worker_piece(spot.total_units, v.workers);
-  const DecodeSpan sp = decode_span<RT>(v, spot.b);
-  const int tile = (int)(at - spot.before), r0 = tile * RT;
-  if (r >= sp.s.n * v.a.group - r0) return;
-  const int64_t from = spot.units_before + (int64_t)tile * sp.units;
-  const int w0 = divide(from, piece), w1 = divide(from + sp.units - 1, piece);
-  if (w0 == w1) return;  // one worker had it all
-  const int64_t size = (int64_t)RT * (c.head + 2);
-  const float* base = v.partial + (int64_t)head * 2 * v.workers * size;
-  // the first worker's range ends inside the tile, the others' begin in it
-  const int first = w0 * piece <= from ? 1 : 0;
-  join_row<RT>(v.a, sp.s, r0, r, head, lane, w1 - w0 + 1,
-               [&](int w) { return base + (2 * (w0 + w) + (w == 0 ? first : 0)) * size; });
+  if (v.partial && head == 0 && tid == 0) v.cuts[blockIdx.x] = cut;
 }
 
 // ---- many rows for each sequence ---------------------------------------------------------------------
@@ -684,12 +627,16 @@ __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(DecodeView
 // Bound: matrix instructions, with the softmax's vector instructions between them.
 constexpr int kStage = 64;
 constexpr int kPromptRows = 128;
+constexpr int kPieces = 1024;     // workgroups that a call with few tiles is cut into, at most,
+constexpr int kMostSplits = 16;   // a tile into as many,
+constexpr int kLeastStages = 4;   // and of so many stages at least
 
 struct PromptView {
   AttentionView a;
-  float* partial;   // [slots][splits][heads][tile rows][head + 2] when splits > 1
-  int slots;        // tiles of rows, at most
-  int splits;
+  float* partial;   // [pieces][heads][tile rows][head + 2], or null: no tile is cut
+  CutTile* cuts;    // [pieces], of the tile whose first piece it is
+  int slots;        // pieces of tiles, at most
+  int pieces;       // wanted, if tiles can be cut
   int rows_from;    // sequences with more packed rows than this are this kernel's
 };
 
@@ -712,13 +659,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   const KvCacheView& c = v.a.c;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int n = lane & 31, h = lane >> 5;
-  const int head = blockIdx.x % c.heads, rest = blockIdx.x / c.heads;
-  const int split = rest % v.splits, slot = v.slots - 1 - rest / v.splits;  // the last tiles of a prompt see the most
-  int64_t index;
-  const int b = kv_find_item(c.batch, slot, lane, &index, [&](int s) { return prompt_tiles(v.a, v.rows_from, s); });
-  if (b < 0) return;
+  const int head = blockIdx.x % c.heads, slot = v.slots - 1 - blockIdx.x / c.heads;  // the last tiles of a prompt see the most
+  int splits = 1;
+  const LineSpot spot = line_find(
+      c.batch, lane, [&](int b) { return (int64_t)prompt_tiles(v.a, v.rows_from, b); },
+      [&](int64_t total) {
+        if (v.partial && 2 * total <= v.pieces) splits = (int)min((uint32_t)v.pieces / max((uint32_t)total, 1u), (uint32_t)kMostSplits);
+        return (int64_t)((uint32_t)slot / (uint32_t)splits);
+      });
+  const int tile = slot / splits, split = slot - tile * splits;
+  const bool notes = v.partial && head == 0 && tid == 0 && slot < v.pieces;
+  if (spot.b < 0) {
+    if (notes) v.cuts[slot] = CutTile{0, 0, 0, 0};
+    return;
+  }
+  const int b = spot.b;
   const KvSequence s = kv_sequence(c, b);
-  const int r0 = __builtin_amdgcn_readfirstlane((int)index) * RT, rows = min(s.n * v.a.group - r0, RT);
+  const int r0 = __builtin_amdgcn_readfirstlane((int)(tile - spot.before)) * RT, rows = min(s.n * v.a.group - r0, RT);
   const int p_first = s.len - s.n + r0 / v.a.group, p_last = s.len - s.n + (r0 + rows - 1) / v.a.group;
   // positions that some row of the tile sees, and that all of them see
   const int lo = v.a.window > 0 ? max(0, p_first - v.a.window + 1) : 0;
@@ -726,8 +683,11 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   const int all_lo = v.a.window > 0 ? max(0, p_last - v.a.window + 1) : 0;
   const int all_hi = v.a.causal ? min(s.len, p_first + 1) : s.len;
   const int u_first = lo / kStage, u_count = max((hi + kStage - 1) / kStage - u_first, 0);
-  const int u0 = u_first + (int)((int64_t)u_count * split / v.splits);
-  const int u1 = u_first + (int)((int64_t)u_count * (split + 1) / v.splits);
+  splits = min(splits, max(u_count / kLeastStages, 1));
+  if (notes) v.cuts[slot] = CutTile{s.row0, r0, split == 0 && splits > 1 ? rows : 0, splits};
+  if (split >= splits) return;
+  const int u0 = u_first + (int)((int64_t)u_count * split / splits);
+  const int u1 = u_first + (int)((int64_t)u_count * (split + 1) / splits);
 
   bf16x8 q[DP / 16];
   int sees_lo, sees_hi;
@@ -852,15 +812,21 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        float y = sc[kt][e] * kscale[buf][32 * kt + 8 * (e >> 2) + 4 * h + (SMALL ? (e & 3) : 0)];
-        if (cap > 0.0f) {
-          const float z = __builtin_amdgcn_exp2f(y * (2.0f * to_log2 / cap));
-          y = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
-        }
-        sc[kt][e] = y;
+        sc[kt][e] *= kscale[buf][32 * kt + 8 * (e >> 2) + 4 * h + (SMALL ? (e & 3) : 0)];
       }
+    if (cap > 0.0f) {
+      KV_CACHE_RARE();
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float z = __builtin_amdgcn_exp2f(sc[kt][e] * (2.0f * to_log2 / cap));
+          sc[kt][e] = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
+        }
+    }
     const bool gap = (there[buf][0] & there[buf][1] & there[buf][2] & there[buf][3]) == 0;
     if (__builtin_amdgcn_readfirstlane((int)(gap || j0 < all_lo || j0 + kStage > all_hi)) != 0) {
+      KV_CACHE_RARE();
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -877,6 +843,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
       for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, sc[kt][e]);
     // the maximum in use may lag behind by up to 2^8, which f32 and bf16 weights bear
     if (__any(most > top + 8.0f)) {
+      KV_CACHE_RARE();
       most = __builtin_fmaxf(most, __shfl_xor(most, 32));
       const float now = __builtin_fmaxf(top, most);
       const float scale = __builtin_amdgcn_exp2f(top - now);
@@ -929,8 +896,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   if (r >= rows) return;
   const int i = (r0 + r) / v.a.group, g = r0 + r - i * v.a.group;
   const int64_t at_row = (int64_t)(s.row0 + i) * v.a.q_heads + head * v.a.group + g;
-  const bool joined = v.splits > 1;
-  float* part = joined ? v.partial + (((int64_t)slot * v.splits + split) * c.heads + head) * RT * (c.head + 2) : nullptr;
+  const bool joined = splits > 1;
+  float* part = joined ? v.partial + ((int64_t)slot * c.heads + head) * RT * (c.head + 2) : nullptr;
   const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
   for (int i2 = 0; i2 < DP / 32; ++i2)
@@ -951,24 +918,75 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   }
 }
 
-// Joins the pieces of a tile of rows; a workgroup for four rows of a tile and head.
-__global__ __launch_bounds__(256) void kv_cache_attention_prompt_join_kernel(PromptView v) {
-  const KvCacheView& c = v.a.c;
-  const int lane = threadIdx.x & 63, head = blockIdx.y, slot = blockIdx.x / (kPromptRows / 4);
-  int64_t index;
-  const int b = kv_find_item(c.batch, slot, lane, &index, [&](int s) { return prompt_tiles(v.a, v.rows_from, s); });
-  if (b < 0) return;
-  const KvSequence s = kv_sequence(c, b);
-  const int r0 = (int)index * kPromptRows;
-  const int r = (blockIdx.x % (kPromptRows / 4)) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (r >= min(s.n * v.a.group - r0, kPromptRows)) return;
-  const float* base = v.partial + ((int64_t)slot * v.splits * c.heads + head) * kPromptRows * (c.head + 2);
-  join_row<kPromptRows>(v.a, s, r0, r, head, lane, v.splits,
-                        [&](int w) { return base + (int64_t)w * c.heads * kPromptRows * (c.head + 2); });
+// ---- the pieces of cut tiles joined --------------------------------------------------------------------
+
+struct JoinPart {
+  const CutTile* cuts;
+  const float* partial;
+  int64_t head_step, cut_step, piece_step;  // floats from head to head, tile to tile, piece to piece
+  int64_t back;     // less for the pieces after the first
+  int tile_rows;
+};
+
+struct JoinView {
+  AttentionView a;
+  JoinPart parts[2];
+  unsigned blocks;  // the first part's
+};
+
+// L lanes for a row, four values each; the pieces in their order.  The maxima and sums of up to L pieces are a lane's
+// each, and the results are under way four pieces at a time.
+// Bound: three dependent reads (the tile's note, the maxima, the results), 6 us with the launch where all is little.
+template <int L>
+__global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(JoinView v) {
+  const JoinPart& p = blockIdx.x < v.blocks ? v.parts[0] : v.parts[1];
+  const int at = (int)(blockIdx.x - (blockIdx.x < v.blocks ? 0u : v.blocks)) * (256 / L);
+  const int size = v.a.c.head, head = blockIdx.y, lane = threadIdx.x & (L - 1);
+  const int item = at / p.tile_rows;
+  const CutTile cut = p.cuts[item];
+  const int r = at % p.tile_rows + (int)threadIdx.x / L;
+  if (r >= cut.rows) return;
+  const float* first = p.partial + head * p.head_step + item * p.cut_step;
+  auto piece = [&](int w) { return first + (w * p.piece_step - (w > 0 ? p.back : 0)); };
+  const int64_t tops = (int64_t)p.tile_rows * size + r;
+  const int d = min(4 * lane, size - 4);
+  float m = -1e30f, l = 0.0f;
+  floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+  for (int w0 = 0; w0 < cut.pieces; w0 += L) {
+    const int here = min(cut.pieces - w0, L);
+    const float* q = piece(w0 + min(lane, here - 1)) + tops;
+    const float top = q[0], sum = q[p.tile_rows];
+    float now = __builtin_fmaxf(m, top);
+#pragma unroll
+    for (int off = L / 2; off > 0; off >>= 1) now = __builtin_fmaxf(now, __shfl_xor(now, off, L));
+    const float old = __builtin_amdgcn_exp2f(m - now);
+    const float scale = lane < here ? __builtin_amdgcn_exp2f(top - now) : 0.0f;
+    m = now;
+    l = l * old + sum * scale;
+    o *= old;
+    for (int w = 0; w < here; w += 4) {
+      floatx4 x[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = *reinterpret_cast<const floatx4*>(piece(w0 + min(w + e, here - 1)) + (int64_t)r * size + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o += x[e] * (w + e < here ? __shfl(scale, w + e, L) : 0.0f);
+    }
+  }
+#pragma unroll
+  for (int off = L / 2; off > 0; off >>= 1) l += __shfl_xor(l, off, L);
+  const int i = (cut.first + r) / v.a.group, g = cut.first + r - i * v.a.group;
+  const int64_t at_row = (int64_t)(cut.row0 + i) * v.a.q_heads + head * v.a.group + g;
+  const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+  if (4 * lane < size)
+    *reinterpret_cast<uintx2*>(v.a.out + at_row * size + d) =
+        uintx2{pack_bf16x2(o[0] * inverse, o[1] * inverse), pack_bf16x2(o[2] * inverse, o[3] * inverse)};
+  if (lane == 0 && v.a.lse) v.a.lse[at_row] = l == 0.0f ? -INFINITY : (m + __builtin_log2f(l)) * 0.693147180559945309f;
 }
 
 // Packed rows of a sequence up to which the streaming kernel takes it in calls that both kernels serve.
 constexpr int kFewRows = 64;
+// Packed rows beyond one row for each sequence up to which the streaming kernel takes a whole call.
+constexpr int kSpareRows = 4096;
 
 // How a call runs, from its shapes alone (lengths are device data).
 struct DecodePlan {
@@ -994,41 +1012,37 @@ DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_h
   if (w > units) w = units;
   d.workers = w < 1 ? 1 : (int)w;
   d.split = positions > kUnit && batch > 0;
-  d.bytes = d.split ? (size_t)(kv_heads * 2 * d.workers * 16 * d.qt * (head + 2)) * 4 : 0;
+  d.bytes = d.split ? (size_t)(d.workers * (sizeof(CutTile) + kv_heads * 2 * 16 * d.qt * (head + 2) * 4)) : 0;
   return d;
 }
 
 struct PromptPlan {
   bool used;
-  int splits;
-  int64_t slots;
+  int pieces;       // 0: no tile is cut
+  int64_t slots;    // pieces of tiles, at most
   size_t bytes;
 };
 
 PromptPlan PlanPrompt(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_heads, int64_t head, int64_t positions) {
   PromptPlan d{};
   const int64_t group = q_heads / kv_heads;
-  d.used = batch > 0 && rows * group > kFewRows && rows > 2 * batch;
+  d.used = batch > 0 && (rows - batch) * group > kSpareRows;
   if (!d.used) return d;
-  d.slots = rows * group / (kPromptRows) + batch;
-  const int64_t stages = (positions + kStage - 1) / kStage;
-  int64_t n = 512 / (d.slots * kv_heads);
-  if (n > stages / 4) n = stages / 4;
-  if (n > 16) n = 16;
-  d.splits = n < 1 ? 1 : (int)n;
-  d.bytes = d.splits > 1 ? (size_t)(d.slots * d.splits * kv_heads * kPromptRows * (head + 2)) * 4 : 0;
+  d.slots = rows * group / kPromptRows + min(batch, rows * group / kFewRows);
+  const int64_t pieces = kPieces / kv_heads;
+  if (rows * group / kPromptRows < pieces && positions >= 2 * kLeastStages * kStage) {
+    d.pieces = (int)pieces;
+    if (d.slots < pieces) d.slots = d.slots * kMostSplits < pieces ? d.slots * kMostSplits : pieces;
+    d.bytes = (size_t)pieces * (sizeof(CutTile) + kv_heads * kPromptRows * (head + 2) * 4);
+  }
   return d;
 }
 
 template <bool F8, int DP>
 void LaunchPrompt(const PromptView& v, hipStream_t stream) {
-  const unsigned grid = (unsigned)(v.slots * v.splits * v.a.c.heads);
+  const unsigned grid = (unsigned)(v.slots * v.a.c.heads);
   if (v.a.c.block_log2 < 2) kv_cache_attention_prompt_kernel<F8, DP, true><<<grid, 256, 0, stream>>>(v);
   else kv_cache_attention_prompt_kernel<F8, DP, false><<<grid, 256, 0, stream>>>(v);
-  if (v.splits > 1) {
-    const dim3 join((unsigned)(v.slots * (kPromptRows / 4)), (unsigned)v.a.c.heads);
-    kv_cache_attention_prompt_join_kernel<<<join, 256, 0, stream>>>(v);
-  }
 }
 
 template <bool F8>
@@ -1094,7 +1108,10 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   dv.workers = d.workers;
   dv.rows_to = pr.used ? kFewRows : INT32_MAX;
   const bool scratch = p.workspace && p.workspace_bytes >= d.bytes + pr.bytes;
-  if (d.split && scratch) dv.partial = (float*)p.workspace;
+  if (d.split && scratch) {
+    dv.cuts = (CutTile*)p.workspace;
+    dv.partial = (float*)(dv.cuts + d.workers);
+  }
   const dim3 grid((unsigned)(d.workers + (v.c.rows + 63) / 64), (unsigned)v.c.heads);
   char name[64];
   const bool f8 = p.cache.cache_dtype == XLA_FFI_DataType_F8E4M3FN;
@@ -1102,23 +1119,40 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   SetLastKernel(name);
   if (f8) LaunchDecode<true>(d, dv, grid, stream);
   else LaunchDecode<false>(d, dv, grid, stream);
+  JoinView jv{};
+  jv.a = v;
+  const int lanes = d.dp / 4, join_rows = 256 / lanes;
+  unsigned joins = 0;
   if (dv.partial) {
-    const dim3 join((unsigned)(d.tiles * 4 * d.qt), (unsigned)v.c.heads);
-    if (d.qt == 1) kv_cache_attention_join_kernel<16><<<join, 256, 0, stream>>>(dv);
-    else kv_cache_attention_join_kernel<32><<<join, 256, 0, stream>>>(dv);
+    const int64_t size = (int64_t)16 * d.qt * (v.c.head + 2);
+    // a worker's second piece is the one that begins its tile, the next workers go on in their first
+    jv.parts[0] = JoinPart{dv.cuts, dv.partial + size, 2 * d.workers * size, 2 * size, 2 * size, size, 16 * d.qt};
+    joins = jv.blocks = (unsigned)(d.workers * (16 * d.qt) / join_rows);
   }
   if (pr.used) {
     PromptView pv{};
     pv.a = v;
     pv.slots = (int)pr.slots;
-    pv.splits = scratch ? pr.splits : 1;
-    pv.partial = pv.splits > 1 ? (float*)((char*)p.workspace + d.bytes) : nullptr;
+    pv.pieces = pr.pieces;
     pv.rows_from = kFewRows;
+    if (pr.pieces > 0 && scratch) {
+      pv.cuts = (CutTile*)((char*)p.workspace + d.bytes);
+      pv.partial = (float*)(pv.cuts + pr.pieces);
+      const int64_t size = (int64_t)kPromptRows * (v.c.head + 2);
+      jv.parts[1] = JoinPart{pv.cuts, pv.partial, size, v.c.heads * size, v.c.heads * size, 0, kPromptRows};
+      joins += (unsigned)(min(pr.slots, (int64_t)pr.pieces) * kPromptRows / join_rows);
+    }
     snprintf(name, sizeof(name), "kv_cache_attention_prompt_%s_d%d_m%d%s", f8 ? "f8" : "s8", d.dp, kPromptRows,
-             pv.splits > 1 ? "_split" : "");
+             pv.partial ? "_split" : "");
     SetLastKernel(name);
     if (f8) LaunchPrompt<true>(d.dp, pv, stream);
     else LaunchPrompt<false>(d.dp, pv, stream);
+  }
+  if (joins > 0) {
+    const dim3 grid((unsigned)joins, (unsigned)v.c.heads);
+    if (d.dp == 64) kv_cache_attention_join_kernel<16><<<grid, 256, 0, stream>>>(jv);
+    else if (d.dp == 128) kv_cache_attention_join_kernel<32><<<grid, 256, 0, stream>>>(jv);
+    else kv_cache_attention_join_kernel<64><<<grid, 256, 0, stream>>>(jv);
   }
   return CheckLaunch("kv_cache_attention");
 }
