@@ -188,6 +188,8 @@ __device__ __forceinline__ void columns(const uint32_t (&k)[8][N], bf16x8& first
 // Keeps what follows in its branch: work that few steps need is not done by all of them and thrown away.
 #define KV_CACHE_INLINE __attribute__((always_inline))  // of a lambda: its captures stay in registers
 #define KV_CACHE_RARE() asm volatile("")
+// Steps of products and what is to run meanwhile stay side by side.
+#define KV_CACHE_FENCE() __builtin_amdgcn_sched_barrier(0)
 
 // Rows first to first + 63, where they belong to no sequence: 0, lse -infinity.
 __device__ void clear_rows_of_nobody(const AttentionView& v, int first) {
@@ -619,17 +621,26 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
 //   S^T = K Q^T   column n of the result is a row of q, a lane holds positions 8 j + 4 h + i
 //   O^T = V^T P^T where the values lie in LDS in that same order of positions, so the weights go from one
 //                 product into the next without leaving their lane.
-// Scales, maxima and roundings are as above.
+// Scales and roundings are as above.
+//
+// A stage goes in halves of 32 positions, so that vector instructions stand in the shadow of matrix instructions: the
+// second half's scores run among the first half's exponentials, the first half's results among the second half's
+// exponentials, the second half's results among the widening of the next stage.
 //
 // 16-byte pieces of a key row are stored at piece ^ (position & 15), those of a value row at
 // piece ^ ((d ^ d >> 2) & 7): eight lanes that read or write together then meet eight different places.
 //
-// Bound: matrix instructions, with the softmax's vector instructions between them.
+// Bound: two waves share a SIMD, and each needs 1312 cycles of vector instructions (a quarter of them exponentials) and
+// 1024 of matrix instructions for a stage of a head of 128, the matrix pipes being busy for 38% of the time.  8192 rows of
+// 32 heads on 8192 positions, causal: 601 us, 915 TFLOP/s, where a large product of matrices reaches 1357.
 constexpr int kStage = 64;
 constexpr int kPromptRows = 128;
-constexpr int kPieces = 1024;     // workgroups that a call with few tiles is cut into, at most,
-constexpr int kMostSplits = 16;   // a tile into as many,
-constexpr int kLeastStages = 4;   // and of so many stages at least
+// Where a call has few tiles, their positions are cut: into pieces that give kPieces workgroups at most (six chunks of
+// prompts, 312 tiles and heads: 111 us uncut, 94 with 1024, 103 with 2048, 123 with 4096), kMostSplits for a tile, of
+// kLeastStages stages or more.  How many tiles there are is device data, so each workgroup counts them.
+constexpr int kPieces = 1024;
+constexpr int kMostSplits = 16;
+constexpr int kLeastStages = 4;
 
 struct PromptView {
   AttentionView a;
@@ -652,6 +663,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   constexpr int KX = KC < 16 ? KC - 1 : 15;
   constexpr int KN = DP / 64;            // pieces of 16 codes that a lane stages of the keys
   constexpr int VN = DP < 128 ? 1 : DP / 128;  // groups of 8 positions x 4 values that a lane stages
+  constexpr int S = SMALL ? 4 : 1;       // scales of four neighbouring positions
+  constexpr int QK = DP / 16;            // steps of 32 positions' scores, and of their results
+  constexpr int PIECES = 2 * KN + 2 * VN;  // of a lane's staging
   __shared__ uintx4 keys[2][kStage * KC];
   __shared__ uintx4 vals[2][DP * 8];
   __shared__ float kscale[2][kStage], vscale[2][kStage];
@@ -711,20 +725,20 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   const float cap = v.a.softcap;
   const float factor = cap > 0.0f ? v.a.scale : v.a.scale * to_log2;
   const int* table = c.table + (int64_t)b * c.width;
-  const int in_page = (1 << c.page_log2) - 1;
+  const int in_page = (1 << c.page_log2) - 1, in_block = (1 << c.block_log2) - 1;
 
   // Stage: wave w brings positions 16 w to 16 w + 15.  Keys: 16 codes a piece, lane -> (position, piece); values: lane ->
   // (eight positions as S^T orders them, four values).
   uintx4 kraw[KN];
   uint32_t vraw[VN][8];
-  float scale_raw = 0.0f;
-  bool present = false;
+  float ks_raw, vs_raw;
+  bool present;
   const int kpos = lane / (DP / 16), kpiece = lane % (DP / 16);  // 64 / (DP / 16) positions at once
   const int vquad = lane % (DP < 128 ? DP / 4 : 32), vhalf = DP < 128 ? (lane / (DP / 4)) & 1 : h;
-  auto page_of = [&](int u) {
+  auto page_of = [&](int u) KV_CACHE_INLINE {
     return const_int(table, min(u * kStage + 16 * wave, hi - 1) >> c.page_log2);
   };
-  auto fetch = [&](int u, int page) {
+  auto fetch = [&](int u, int page) KV_CACHE_INLINE {
     const int j = u * kStage + 16 * wave;
     present = (unsigned)page < (unsigned)c.pages && u < u1 && j < hi && j + 16 > lo;
     page = present ? page : 0;  // read, and masked
@@ -741,10 +755,14 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
       for (int e = 0; e < 8; ++e)
         vraw[i][e] = *reinterpret_cast<const uint32_t*>(
             vp + (uint32_t)((8 * (e >> 2) + 4 * vhalf + (e & 3)) * c.head + min(128 * i + 4 * vquad, c.head - 4)));
-    const int64_t sc = kv_scale(c, page, head, row + (lane & 15));
-    scale_raw = c.scales[(lane >> 4) & 1][sc];
+    const int64_t sc = kv_scale(c, page, head, row);
+    const float* ksp = c.scales[0] + sc;
+    const float* vsp = c.scales[1] + sc;
+    const uint32_t place = (uint32_t)((row & in_block) + (lane & 15)) >> c.block_log2;
+    ks_raw = ksp[place];
+    vs_raw = vsp[place];
   };
-  auto stage = [&](int u, int buf) {
+  auto stage_scales = [&](int u, int buf) KV_CACHE_INLINE {
     const int j0 = u * kStage + 16 * wave;
     if (F8 && (!present || j0 < lo || j0 + 16 > hi)) {
       KV_CACHE_RARE();
@@ -756,34 +774,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
         for (int i = 0; i < VN; ++i) vraw[i][e] = present && j >= lo && j < hi ? vraw[i][e] : 0u;
       }
     }
-#pragma unroll
-    for (int i = 0; i < KN; ++i) {
-      const int pos = 16 * wave + i * (1024 / DP) + kpos;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uintx4 w;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          w[2 * e] = widen2<F8, 0>(kraw[i][2 * half + e]);
-          w[2 * e + 1] = widen2<F8, 2>(kraw[i][2 * half + e]);
-        }
-        keys[buf][pos * KC + ((2 * kpiece + half) ^ (pos & KX))] = w;
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < VN; ++i) {
-      uint32_t one[8][1];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) one[e][0] = vraw[i][e];
-      static_for<0, 2>([&](auto t) {
-        const int d = 128 * i + 4 * vquad + 2 * decltype(t)::value;
-        bf16x8 va, vb;
-        columns<F8, 2 * decltype(t)::value>(one, va, vb);
-        vals[buf][d * 8 + ((2 * wave + vhalf) ^ ((d ^ (d >> 2)) & 7))] = __builtin_bit_cast(uintx4, va);
-        vals[buf][d * 8 + 8 + ((2 * wave + vhalf) ^ (((d + 1) ^ (d >> 2)) & 7))] = __builtin_bit_cast(uintx4, vb);
-      });
-    }
-    float ks = scale_raw, vs = __shfl_xor(scale_raw, 16);  // lanes 0 to 15: of position 16 wave + lane
+    float ks = ks_raw, vs = vs_raw;
     keep_to_its_rows(ks, vs);
     if (lane < 16) {
       kscale[buf][16 * wave + lane] = ks * factor;
@@ -791,59 +782,104 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     }
     if (lane == 0) there[buf][wave] = present ? 1 : 0;
   };
+  auto stage_piece = [&](auto at, int buf) KV_CACHE_INLINE {
+    constexpr int P = decltype(at)::value;
+    if constexpr (P < 2 * KN) {
+      constexpr int I = P / 2, H = P % 2;
+      const int pos = 16 * wave + I * (1024 / DP) + kpos;
+      keys[buf][pos * KC + ((2 * kpiece + H) ^ (pos & KX))] = __builtin_bit_cast(uintx4, widen8<F8>(kraw[I][2 * H], kraw[I][2 * H + 1]));
+    } else {
+      constexpr int I = (P - 2 * KN) / 2, T = 2 * ((P - 2 * KN) % 2);
+      const int d = 128 * I + 4 * vquad + T;
+      uint32_t one[8][1];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) one[e][0] = vraw[I][e];
+      bf16x8 va, vb;
+      columns<F8, T>(one, va, vb);
+      vals[buf][d * 8 + ((2 * wave + vhalf) ^ ((d ^ (d >> 2)) & 7))] = __builtin_bit_cast(uintx4, va);
+      vals[buf][d * 8 + 8 + ((2 * wave + vhalf) ^ (((d + 1) ^ (d >> 2)) & 7))] = __builtin_bit_cast(uintx4, vb);
+    }
+  };
 
-  auto work = [&](int u, int buf, auto between) {
-    const int j0 = u * kStage;
-    floatx16 sc[2];
+  floatx16 sc[2];
+  bf16x8 p[2][2];
+  float kq[4 * S], vq[4 * S], more;
+  auto key_piece = [&](int buf, int kt, int k) KV_CACHE_INLINE {
+    const int pos = 32 * kt + n;
+    return __builtin_bit_cast(bf16x8, keys[buf][pos * KC + ((2 * k + h) ^ (pos & KX))]);
+  };
+  auto value_piece = [&](int buf, int kt, int at) KV_CACHE_INLINE {  // at: which 16 positions, then which 32 values
+    const int g = 2 * kt + at / (DP / 32), d = 32 * (at % (DP / 32)) + n;
+    return __builtin_bit_cast(bf16x8, vals[buf][d * 8 + ((2 * g + h) ^ ((d ^ (d >> 2)) & 7))]);
+  };
+  auto score = [&](auto kt_, bf16x8 a, auto k_) KV_CACHE_INLINE {
+    constexpr int KT = decltype(kt_)::value, K = decltype(k_)::value;
+    floatx16 from = sc[KT];
+    if constexpr (K == 0) {
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+      for (int e = 0; e < 16; ++e) from[e] = 0.0f;
+    }
+    sc[KT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[K], from, 0, 0, 0);
+  };
+  auto result = [&](auto kt_, bf16x8 a, auto at_) KV_CACHE_INLINE {
+    constexpr int KT = decltype(kt_)::value, G = decltype(at_)::value / (DP / 32), I = decltype(at_)::value % (DP / 32);
+    acc[I] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p[KT][G], acc[I], 0, 0, 0);
+  };
+  // The scales of a half; where scores are capped or some position is not seen, the scores themselves are made final.
+  auto prepare = [&](bool edge, int buf, int j0, auto kt_) KV_CACHE_INLINE {
+    constexpr int KT = decltype(kt_)::value;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[kt][e] = 0.0f;
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const int pos = 32 * kt + n;
-        const bf16x8 a = __builtin_bit_cast(bf16x8, keys[buf][pos * KC + ((2 * k + h) ^ (pos & KX))]);
-        sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[k], sc[kt], 0, 0, 0);
-      }
-    between();
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        sc[kt][e] *= kscale[buf][32 * kt + 8 * (e >> 2) + 4 * h + (SMALL ? (e & 3) : 0)];
-      }
+    for (int i = 0; i < 4 * S; ++i) {
+      const int pos = 32 * KT + 8 * (i / S) + 4 * h + i % S;
+      kq[i] = kscale[buf][pos];
+      vq[i] = vscale[buf][pos];
+    }
     if (cap > 0.0f) {
       KV_CACHE_RARE();
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int r = 0; r < 16; ++r) {
+        const float z = __builtin_amdgcn_exp2f(sc[KT][r] * kq[(r >> 2) * S + (r & (S - 1))] * (2.0f * to_log2 / cap));
+        sc[KT][r] = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
+      }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float z = __builtin_amdgcn_exp2f(sc[kt][e] * (2.0f * to_log2 / cap));
-          sc[kt][e] = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
-        }
+      for (int i = 0; i < 4 * S; ++i) kq[i] = 1.0f;
     }
-    const bool gap = (there[buf][0] & there[buf][1] & there[buf][2] & there[buf][3]) == 0;
-    if (__builtin_amdgcn_readfirstlane((int)(gap || j0 < all_lo || j0 + kStage > all_hi)) != 0) {
+    if (edge) {
       KV_CACHE_RARE();
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int r = 0; r < 16; ++r) {
+        const int pos = j0 + 32 * KT + 8 * (r >> 2) + 4 * h + (r & 3);
+        const bool seen = there[buf][2 * KT + (r >> 3)] != 0 && pos >= sees_lo && pos < sees_hi;
+        sc[KT][r] = seen ? sc[KT][r] * kq[(r >> 2) * S + (r & (S - 1))] : -INFINITY;
+      }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int pos = j0 + 32 * kt + 8 * (e >> 2) + 4 * h + (e & 3);
-          const bool seen = there[buf][2 * kt + (e >> 3)] != 0 && pos >= sees_lo && pos < sees_hi;
-          sc[kt][e] = seen ? sc[kt][e] : -INFINITY;
-        }
+      for (int i = 0; i < 4 * S; ++i) kq[i] = 1.0f;
     }
-    float most = sc[0][0];
+  };
+  // the weights of positions 8 I + 4 h to + 3 of a half
+  auto weigh = [&](auto kt_, auto unit) KV_CACHE_INLINE {
+    constexpr int KT = decltype(kt_)::value, I = decltype(unit)::value;
+    float w[4];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt)
+    for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[KT][4 * I + e], kq[I * S + (e & (S - 1))], -top));
+    const float four = (w[0] + w[1]) + (w[2] + w[3]);
+    more = I == 0 ? four : more + four;
 #pragma unroll
-      for (int e = 0; e < 16; ++e) most = __builtin_fmaxf(most, sc[kt][e]);
-    // the maximum in use may lag behind by up to 2^8, which f32 and bf16 weights bear
-    if (__any(most > top + 8.0f)) {
+    for (int e = 0; e < 4; ++e) w[e] *= vq[I * S + (e & (S - 1))];
+    uintx4 packed = I & 1 ? __builtin_bit_cast(uintx4, p[KT][I >> 1]) : uintx4{0u, 0u, 0u, 0u};
+    packed[2 * (I & 1)] = pack_bf16x2(w[0], w[1]);
+    packed[2 * (I & 1) + 1] = pack_bf16x2(w[2], w[3]);
+    p[KT][I >> 1] = __builtin_bit_cast(bf16x8, packed);
+  };
+  // The maximum in use may lag behind by up to 2^10, which f32 and bf16 weights bear; where the weights' sum shows
+  // more, the half is weighed again.
+  auto catch_up = [&](auto kt_) KV_CACHE_INLINE {
+    constexpr int KT = decltype(kt_)::value;
+    if (__any(more > 1024.0f)) {
       KV_CACHE_RARE();
+      float most = -INFINITY;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, sc[KT][r] * kq[(r >> 2) * S + (r & (S - 1))]);
       most = __builtin_fmaxf(most, __shfl_xor(most, 32));
       const float now = __builtin_fmaxf(top, most);
       const float scale = __builtin_amdgcn_exp2f(top - now);
@@ -851,42 +887,74 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
       sum *= scale;
 #pragma unroll
       for (int i = 0; i < DP / 32; ++i) acc[i] *= scale;
+      static_for<0, 4>([&](auto unit) KV_CACHE_INLINE { weigh(kt_, unit); });
     }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-      uintx4 w;
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const int r = 8 * (g & 1) + e, pos = 32 * (g >> 1) + 8 * (r >> 2) + 4 * h;
-        const float p0 = __builtin_amdgcn_exp2f(sc[g >> 1][r] - top), p1 = __builtin_amdgcn_exp2f(sc[g >> 1][r + 1] - top);
-        sum += p0 + p1;
-        w[e >> 1] = pack_bf16x2(p0 * vscale[buf][pos + (SMALL ? (r & 3) : 0)], p1 * vscale[buf][pos + (SMALL ? (r & 3) + 1 : 0)]);
-      }
-      const bf16x8 p = __builtin_bit_cast(bf16x8, w);
-#pragma unroll
-      for (int i = 0; i < DP / 32; ++i) {
-        const int d = 32 * i + n;
-        const bf16x8 a = __builtin_bit_cast(bf16x8, vals[buf][d * 8 + ((2 * g + h) ^ ((d ^ (d >> 2)) & 7))]);
-        acc[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p, acc[i], 0, 0, 0);
-      }
-    }
+    sum += more;
   };
+  constexpr std::integral_constant<int, 0> kFirst{};
+  constexpr std::integral_constant<int, 1> kSecond{};
 
   if (u0 < u1) {
     fetch(u0, page_of(u0));
-    stage(u0, 0);
+    stage_scales(u0, 0);
+    static_for<0, PIECES>([&](auto at) KV_CACHE_INLINE { stage_piece(at, 0); });
     int next = page_of(u0 + 2);
     fetch(u0 + 1, page_of(u0 + 1));
     __syncthreads();
     for (int u = u0; u < u1; ++u) {
-      const int buf = (u - u0) & 1;
-      work(u, buf, [&] {
-        if (u + 1 < u1) {
-          stage(u + 1, buf ^ 1);
-          fetch(u + 2, next);
-          next = page_of(u + 3);
-        }
-      });
+      const int buf = (u - u0) & 1, j0 = u * kStage;
+      {
+        bf16x8 a = key_piece(buf, 0, 0);
+        static_for<0, QK>([&](auto k) KV_CACHE_INLINE {
+          constexpr int K = decltype(k)::value;
+          const bf16x8 now = a;
+          if constexpr (K + 1 < QK) a = key_piece(buf, 0, K + 1);
+          score(kFirst, now, k);
+        });
+      }
+      const bool gap = (there[buf][0] & there[buf][1] & there[buf][2] & there[buf][3]) == 0;
+      const bool edge = __builtin_amdgcn_readfirstlane((int)(gap || j0 < all_lo || j0 + kStage > all_hi)) != 0;
+      prepare(edge, buf, j0, kFirst);
+      {
+        bf16x8 a = key_piece(buf, 1, 0);
+        static_for<0, QK>([&](auto k) KV_CACHE_INLINE {
+          constexpr int K = decltype(k)::value;
+          const bf16x8 now = a;
+          if constexpr (K + 1 < QK) a = key_piece(buf, 1, K + 1);
+          score(kSecond, now, k);
+          static_for<K * 4 / QK, (K + 1) * 4 / QK>([&](auto unit) KV_CACHE_INLINE { weigh(kFirst, unit); });
+          KV_CACHE_FENCE();
+        });
+      }
+      catch_up(kFirst);
+      prepare(edge, buf, j0, kSecond);
+      {
+        bf16x8 a = value_piece(buf, 0, 0);
+        static_for<0, QK>([&](auto k) KV_CACHE_INLINE {
+          constexpr int K = decltype(k)::value;
+          const bf16x8 now = a;
+          if constexpr (K + 1 < QK) a = value_piece(buf, 0, K + 1);
+          result(kFirst, now, k);
+          static_for<K * 4 / QK, (K + 1) * 4 / QK>([&](auto unit) KV_CACHE_INLINE { weigh(kSecond, unit); });
+          KV_CACHE_FENCE();
+        });
+      }
+      catch_up(kSecond);
+      // past the last stage, of whatever is there
+      stage_scales(u + 1, buf ^ 1);
+      {
+        bf16x8 a = value_piece(buf, 1, 0);
+        static_for<0, QK>([&](auto k) KV_CACHE_INLINE {
+          constexpr int K = decltype(k)::value;
+          const bf16x8 now = a;
+          if constexpr (K + 1 < QK) a = value_piece(buf, 1, K + 1);
+          result(kSecond, now, k);
+          static_for<K * PIECES / QK, (K + 1) * PIECES / QK>([&](auto at) KV_CACHE_INLINE { stage_piece(at, buf ^ 1); });
+          KV_CACHE_FENCE();
+        });
+      }
+      fetch(u + 2, next);
+      next = page_of(u + 3);
       __syncthreads();
     }
   }
@@ -936,7 +1004,7 @@ struct JoinView {
 
 // L lanes for a row, four values each; the pieces in their order.  The maxima and sums of up to L pieces are a lane's
 // each, and the results are under way four pieces at a time.
-// Bound: three dependent reads (the tile's note, the maxima, the results), 6 us with the launch where all is little.
+// Bound: three dependent reads (the tile's note, the maxima, the results): 4.4 us for one sequence's 64 rows, 4.9 for 64.
 template <int L>
 __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(JoinView v) {
   const JoinPart& p = blockIdx.x < v.blocks ? v.parts[0] : v.parts[1];
@@ -985,8 +1053,11 @@ __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(JoinView v
 
 // Packed rows of a sequence up to which the streaming kernel takes it in calls that both kernels serve.
 constexpr int kFewRows = 64;
-// Packed rows beyond one row for each sequence up to which the streaming kernel takes a whole call.
-constexpr int kSpareRows = 4096;
+// Packed rows beyond one row for each sequence up to which the streaming kernel takes a whole call, since two
+// kernels one after the other each have an end at which little runs.  32 heads on 8 of 128, streaming alone and both:
+// 63 single rows and one chunk of 512 on 4096 positions (2044 to spare) 167 and 187 us, a prompt of 512 25 and 40;
+// 64 x 17 rows on 4096 (4096 to spare) 308 and 222, a prompt of 2048 (8188) 168 and 93.
+constexpr int kSpareRows = 2048;
 
 // How a call runs, from its shapes alone (lengths are device data).
 struct DecodePlan {
