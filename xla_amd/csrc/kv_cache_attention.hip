@@ -303,8 +303,8 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
   const int vread = 32 * DP + (16 * (vrow >> 2) + 4 * grp + (vrow & 3)) * DP + ((vrow & KX) << 4) + 8 * (lane & 1);
   const float to_log2 = 1.44269504088896341f;
   const float cap = v.a.softcap;
-  // scores in units of log 2: exp2 takes them as they are
-  const float factor = cap > 0.0f ? v.a.scale : v.a.scale * to_log2;
+  // scores in units of log 2, which exp2 takes as they are, or of cap / 2 log 2: cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap))
+  const float factor = v.a.scale * (cap > 0.0f ? 2.0f * to_log2 / cap : to_log2);
   const int in_page = (1 << c.page_log2) - 1;
 
   while (b >= 0 && b < c.batch && pos < stop) {
@@ -491,12 +491,9 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
         for (int e = 0; e < 8; ++e) y[e] = s[t][e >> 2][e & 3] * (ks[e >> 2][SMALL ? (e & 3) : 0] * factor);
         if (cap > 0.0f) {
           KV_CACHE_RARE();
-          // cap * tanh(y / cap), in units of log 2
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float z = __builtin_amdgcn_exp2f(y[e] * (2.0f * to_log2 / cap));
-            y[e] = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
-          }
+          for (int e = 0; e < 8; ++e)
+            y[e] = __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(y[e])), -2.0f * cap * to_log2, cap * to_log2);
         }
         if (edge) {
           KV_CACHE_RARE();
@@ -723,7 +720,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.0f;
   const float to_log2 = 1.44269504088896341f;
   const float cap = v.a.softcap;
-  const float factor = cap > 0.0f ? v.a.scale : v.a.scale * to_log2;
+  // scores in units of log 2, which exp2 takes as they are, or of cap / 2 log 2: cap tanh(x / cap) = cap - 2 cap / (1 + e^(2 x / cap))
+  const float factor = v.a.scale * (cap > 0.0f ? 2.0f * to_log2 / cap : to_log2);
   const int* table = c.table + (int64_t)b * c.width;
   const int in_page = (1 << c.page_log2) - 1, in_block = (1 << c.block_log2) - 1;
 
@@ -838,8 +836,8 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
       KV_CACHE_RARE();
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const float z = __builtin_amdgcn_exp2f(sc[KT][r] * kq[(r >> 2) * S + (r & (S - 1))] * (2.0f * to_log2 / cap));
-        sc[KT][r] = (cap * to_log2) * (1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + z));
+        const float z = __builtin_amdgcn_exp2f(sc[KT][r] * kq[(r >> 2) * S + (r & (S - 1))]);
+        sc[KT][r] = __builtin_fmaf(__builtin_amdgcn_rcpf(1.0f + z), -2.0f * cap * to_log2, cap * to_log2);
       }
 #pragma unroll
       for (int i = 0; i < 4 * S; ++i) kq[i] = 1.0f;
