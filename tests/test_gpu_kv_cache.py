@@ -54,7 +54,7 @@ def offsets(new, start=0):
     return np.concatenate([[start], start + np.cumsum(new)]).astype(np.int32)
 
 
-def check_attention(pool, q, q_offsets, *, lse=True, scratch="auto", **kw):
+def check_attention(pool, q, q_offsets, *, lse=True, scratch="auto", tiny=0.0, **kw):
     print("attention", pool.kind, q.shape, pool.k.shape, pool.block, pool.lens.tolist()[:8], kw, flush=True)
     qt, qf = bf16(q)
     scale = kw.pop("scale", q.shape[2] ** -0.5)
@@ -64,7 +64,7 @@ def check_attention(pool, q, q_offsets, *, lse=True, scratch="auto", **kw):
                                                   q_offsets, np.float32(scale), **kw)
     tol, tol_lse = plain.attention_tolerance(ref, ref_lse, spread, slack, int(pool.lens.max(initial=0)))
     got = out.float().cpu().numpy().astype(np.float64)
-    bad = ~(np.abs(got - ref) <= tol)
+    bad = ~(np.abs(got - ref) <= tol + tiny)
     assert not bad.any(), (int(bad.sum()), bad.size, [(tuple(i), got[tuple(i)], ref[tuple(i)], tol[tuple(i)]) for i in np.argwhere(bad)[:4]])
     g = got_lse.cpu().numpy().astype(np.float64)
     none = np.isneginf(ref_lse)
@@ -118,6 +118,85 @@ def test_prompts(kind, head, group, n, causal):
     check_attention(pool, q, offsets(new), causal=causal)
     if causal:
         check_attention(pool, q, offsets(new), window=65, softcap=10.0)
+
+
+# (head, heads, group, page, block, new, lens): many more packed rows than sequences, so that the kernel of the prompts
+# takes part; its tiles are of 128 packed rows, its stages of 64 positions
+PROMPTS = [(128, 2, 16, 64, 16, [140, 1, 33, 3], [140, 700, 210, 65]), (64, 1, 32, 16, 1, [70, 9], [70, 333]),
+           (80, 1, 40, 32, 2, [55, 2, 0, 5], [120, 64, 9, 3]), (128, 1, 64, 16, 2, [36, 4], [1, 129]),
+           (16, 2, 64, 128, 4, [64], [64]), (256, 1, 16, 64, 32, [128, 8, 1], [191, 8, 63]), (208, 1, 24, 16, 1, [87, 5], [900, 5]),
+           (96, 3, 24, 256, 256, [100], [257]), (64, 2, 3, 64, 64, [700, 1, 65], [1500, 3, 65])]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("scratch", ["auto", None])
+@pytest.mark.parametrize("head, heads, group, page, block, new, lens", PROMPTS)
+def test_prompts_of_many_heads(kind, scratch, head, heads, group, page, block, new, lens):
+    """Also sequences with fewer positions than rows, and rows of nobody at both ends."""
+    rng = np.random.default_rng(head + group)
+    pool = Pool(rng, kind, lens, heads, head, page, block)
+    q = rng.standard_normal((sum(new) + 3, heads * group, head))
+    for kw in (dict(), dict(causal=False), dict(window=50), dict(window=1), dict(window=130, softcap=3.0), dict(causal=False, softcap=20.0)):
+        a = check_attention(pool, q, offsets(new, 1), scratch=scratch, **kw)
+        assert ffi.last_kernel().startswith("kv_cache_attention_prompt")
+    b = check_attention(pool, q, offsets(new, 1), scratch=scratch, **kw)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+@pytest.mark.parametrize("new, lens", [([40] * 70, [40 + 3 * i for i in range(70)]), ([1] * 90 + [300], [64 + i for i in range(91)]),
+                                       ([8] * 40, [2000] * 40), ([1100], [1100]), ([129, 0, 1, 258, 20], [4100, 0, 3000, 2300, 20])])
+def test_tiles_cut_and_whole(new, lens):
+    """More tiles than are worth cutting, few among many single rows, pieces of very different lengths."""
+    rng = np.random.default_rng(len(new))
+    pool = Pool(rng, "f8", lens, 2, 64, 64, 16)
+    q = rng.standard_normal((sum(new), 2 * 8, 64))
+    check_attention(pool, q, offsets(new))
+    assert ffi.last_kernel().startswith("kv_cache_attention_prompt")
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("head, group, new", [(128, 4, [1, 2, 20]), (64, 32, [1, 90, 4]), (128, 32, [70, 2, 3]), (256, 16, [150, 1, 3])])
+@pytest.mark.parametrize("block", [1, 16])
+def test_scales_of_every_size(kind, head, group, new, block):
+    """Blocks whose scales are zero, negative, tiny, subnormal or large, in both kernels.  A weight times its value's
+    scale that is below 2^-126 may become zero: 2^-126 times a code, for each position; the weights' sum is 1 or more."""
+    rng = np.random.default_rng(head + group)
+    pool = Pool(rng, kind, [90, 300, 20], 2, head, 16, block)
+    shape = pool.ks.shape
+    pool.vs *= rng.choice([1.0, 0.0, -1.0, 1e-30, 1e-42, 1e-3, 50.0], shape).astype(np.float32)
+    pool.ks *= rng.choice([1.0, 0.0, -1.0, 1e-30, 1e-42, 1e-3, 3.0], shape).astype(np.float32)
+    q = rng.standard_normal((sum(new), 2 * group, head))
+    check_attention(pool, q, offsets(new), tiny=300 * 448 * 2.0 ** -126)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group", [2, 64])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_value_scale_that_is_no_number(kind, group, bad):
+    """It reaches the result and the lse of the rows that see it, and no others, in both kernels."""
+    rng = np.random.default_rng(5)
+    pool = Pool(rng, kind, [64], 1, 128, 64, 16)
+    pool.vs[pool.table[0, 0], 0, 2] = bad          # positions 32 to 47
+    q = rng.standard_normal((64, group, 128))
+    out, lse = ops.kv_cache_attention(bf16(q)[0], *pool.device(), dev(offsets([64])), lse=True)
+    assert ffi.last_kernel().startswith("kv_cache_attention_prompt") == (group == 64)
+    assert torch.isnan(out[32:]).all() and torch.isnan(lse[32:]).all()
+    assert torch.isfinite(out[:32]).all() and torch.isfinite(lse[:32]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_maxima_that_grow_along_the_keys(kind):
+    """Scores that rise by far more than a weight bears, from stage to stage, half to half and block to block."""
+    rng = np.random.default_rng(7)
+    pool = Pool(rng, kind, [640], 1, 64, 64, 4)
+    pool.k[:] = np.abs(pool.k) if kind == "s8" else pool.k & 0x7f
+    pool.ks *= (2.0 ** np.arange(pool.ks.shape[2]) / 64).astype(np.float32)
+    order = rng.permutation(pool.ks.shape[2])
+    q = np.abs(rng.standard_normal((100, 64, 64)))
+    check_attention(pool, q, offsets([100]))
+    check_attention(pool, -q, offsets([100]))
+    pool.ks = np.ascontiguousarray(pool.ks[:, :, order])
+    check_attention(pool, q, offsets([100]))
 
 
 @pytest.mark.parametrize("kind", KINDS)

@@ -141,7 +141,7 @@ __device__ __forceinline__ int64_t worker_piece(int64_t total, int workers) {
 }
 
 __device__ __forceinline__ int divide(int64_t x, int64_t by) {
-  return (uint64_t)x < (1ull << 31) ? (int)((uint32_t)x / (uint32_t)by) : (int)(x / by);
+  return (uint64_t)(x | by) < (1ull << 31) ? (int)((uint32_t)x / (uint32_t)by) : (int)(x / by);
 }
 
 // Two codes at byte places i, i + 1 -> two bf16 in a dword, exact.
@@ -1155,7 +1155,8 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   if (!(p.softcap >= 0.0f) || !(p.softcap < INFINITY)) return Fail(kBad, "kv_cache_attention: softcap must be a number that is not negative");
   if (!(p.softmax_scale > -INFINITY && p.softmax_scale < INFINITY))
     return Fail(kBad, "kv_cache_attention: softmax_scale must be a number");
-  if (p.cache.rows * p.q_heads > INT32_MAX) return Fail(kBad, "kv_cache_attention: at most 2^31 - 1 rows times heads");
+  // (a grid holds fewer than 2^32 threads: 256 for every 128 packed rows, and for every sequence of 64 and more)
+  if (p.cache.rows * p.q_heads > 1 << 29) return Fail(kBad, "kv_cache_attention: at most 2^29 rows times heads");
   if (v.c.rows > 0 && (!p.q || !p.out)) return Fail(kBad, "kv_cache_attention: null q or out");
   if ((((uintptr_t)p.q | (uintptr_t)p.out | (uintptr_t)p.workspace) & 15) != 0 || ((uintptr_t)p.lse & 3) != 0)
     return Fail(kBad, "kv_cache_attention: q, out and scratch must be aligned to 16 bytes, lse to 4");

@@ -318,6 +318,7 @@ size_t Align16(size_t x) { return (x + 15) & ~(size_t)15; }
 struct CopyView {
   const int* moves;
   int pages, buffers, parts;  // parts: of the large buffers together
+  int64_t items;
   uint8_t* base[XLA_AMD_KV_CACHE_MAX_BUFFERS];
   int64_t bytes[XLA_AMD_KV_CACHE_MAX_BUFFERS];
 };
@@ -325,6 +326,7 @@ struct CopyView {
 // A workgroup copies kCopyPart bytes of one page of a large buffer, each thread four loads and then four stores
 // (one in flight a thread left 4.8 of the 6.5 TB/s that a plain copy reaches), or the pages of all small buffers.
 constexpr int kCopyPart = 16384, kCopySmall = 4096;
+constexpr int64_t kCopyGrid = 1 << 22;  // workgroups; a longer list of moves goes round again
 
 template <class T, int N>
 __device__ __forceinline__ void copy_part(uint8_t* dst, const uint8_t* src, int64_t bytes, int first, int step) {
@@ -348,9 +350,8 @@ __device__ __forceinline__ void copy_bytes(uint8_t* dst, const uint8_t* src, int
   else copy_part<uint8_t, 4>(dst, src, bytes, first, step);
 }
 
-__global__ __launch_bounds__(256) void kv_cache_copy_pages_kernel(CopyView v) {
-  const int move = blockIdx.x / (v.parts + 1), part = blockIdx.x % (v.parts + 1);
-  const int64_t src = const_int(v.moves, 2 * (int64_t)move), dst = const_int(v.moves, 2 * (int64_t)move + 1);
+__device__ __forceinline__ void copy_item(const CopyView& v, int64_t move, int part) {
+  const int64_t src = const_int(v.moves, 2 * move), dst = const_int(v.moves, 2 * move + 1);
   if ((uint64_t)src >= (uint64_t)v.pages || (uint64_t)dst >= (uint64_t)v.pages || src == dst) return;
   if (part == v.parts) {
     // the small buffers, a wave each
@@ -369,6 +370,12 @@ __global__ __launch_bounds__(256) void kv_cache_copy_pages_kernel(CopyView v) {
   const int64_t bytes = v.bytes[buffer], from = (int64_t)at * kCopyPart;
   copy_bytes(v.base[buffer] + dst * bytes + from, v.base[buffer] + src * bytes + from, min(bytes - from, (int64_t)kCopyPart),
              (uint64_t)(uintptr_t)v.base[buffer] | (uint64_t)bytes, threadIdx.x, 256);
+}
+
+__global__ __launch_bounds__(256) void kv_cache_copy_pages_kernel(CopyView v) {
+  const unsigned per = (unsigned)v.parts + 1;
+  copy_item(v, blockIdx.x / per, (int)(blockIdx.x % per));
+  for (int64_t i = (int64_t)blockIdx.x + gridDim.x; i < v.items; i += gridDim.x) copy_item(v, i / per, (int)(i % per));
 }
 
 }  // namespace
@@ -486,11 +493,10 @@ int LaunchKvCacheCopyPages(const XlaAmdKvCacheCopyPages& p, hipStream_t stream) 
     if (v.bytes[i] > kCopySmall) parts += (v.bytes[i] + kCopyPart - 1) / kCopyPart;
   }
   if (p.num_moves == 0 || p.pages == 0 || most == 0) return 0;
-  if ((parts + 1) * p.num_moves > INT32_MAX)
-    return Fail(kBad, "kv_cache_copy_pages: at most 2^31 - 1 moves times parts of %d bytes", kCopyPart);
-  v.parts = (int)parts;
+  v.parts = (int)parts;  // at most 64 buffers of 2^17 each
+  v.items = (parts + 1) * p.num_moves;  // below 2^23 * 2^31
   SetLastKernel("kv_cache_copy_pages");
-  kv_cache_copy_pages_kernel<<<(unsigned)((parts + 1) * p.num_moves), 256, 0, stream>>>(v);
+  kv_cache_copy_pages_kernel<<<(unsigned)(v.items < kCopyGrid ? v.items : kCopyGrid), 256, 0, stream>>>(v);
   return CheckLaunch("kv_cache_copy_pages");
 }
 

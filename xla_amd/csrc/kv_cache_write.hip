@@ -37,9 +37,9 @@ int MakeKvCacheView(const XlaAmdKvCache& p, const char* what, KvCacheView* c) {
     return Fail(kBad, "%s: the head size must be a multiple of 16 from 16 to 256", what);
   if (p.pages < 0 || p.batch < 0 || p.table_width < 0 || p.rows < 0) return Fail(kBad, "%s: negative size", what);
   if (p.kv_heads < 1 || p.kv_heads > 1024) return Fail(kBad, "%s: kv_heads must be 1 to 1024", what);
-  if (p.pages > INT32_MAX || p.rows > (1 << 24) || p.batch > (1 << 20) ||
+  if (p.pages > INT32_MAX || p.rows >= (1 << 24) || p.batch > (1 << 20) ||
       p.table_width > (int64_t)(INT32_MAX - 1024) / p.page_size)
-    return Fail(kBad, "%s: at most 2^31 - 1 pages, 2^24 rows, 2^20 sequences and 2^31 positions", what);
+    return Fail(kBad, "%s: at most 2^31 - 1 pages, 2^24 - 1 rows, 2^20 sequences and 2^31 positions", what);
   if (p.batch > 0 && p.rows > 0) {
     if (!p.kv_lens || !p.q_offsets || (p.table_width > 0 && !p.page_table))
       return Fail(kBad, "%s: null page_table, kv_lens or q_offsets", what);
@@ -184,10 +184,8 @@ __device__ __forceinline__ uintx2 quantise8(uintx4 w, float scale) {
 }
 
 // One wave for a block and head, keys and values together: finding the block and its page costs a wave more than
-// its arithmetic does.  A lane holds HELD groups of eight values of each while the maximum is found (16 rows of 128
+// its arithmetic does.  A lane holds kHeld groups of eight values of each while the maximum is found (16 rows of 128
 // values, or one row of a decode step); a block with more new values reads them again, from L2.
-// 8192 sequences' worth of waves fit the device: 16 prompts of 16352 rows over 8 heads of 128, 16-row blocks, take
-// two rounds of waves less than with a wave for keys and one for values that read twice.
 constexpr int kHeld = 4;
 
 template <bool F8>
