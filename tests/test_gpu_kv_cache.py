@@ -1,5 +1,7 @@
 """The calls over the 8-bit paged key/value cache against their plain restatement: codes, scales and
 book-keeping bit for bit, attention within bounds that follow from its roundings (oracle/kv_cache.py)."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -532,6 +534,33 @@ def test_copy_pages_of_every_type_and_size():
 
 # ---- as a program uses them ------------------------------------------------------------------------
 
+def test_copy_pages_unaligned_and_large():
+    """Pages of sizes and at addresses that no wide access fits, larger and smaller than a workgroup's part."""
+    rng = np.random.default_rng(89)
+    buffers, want = [], []
+    for size, shift in ((1, 0), (4095, 1), (4097, 3), (16385, 0), (40000, 4), (33000, 1), (20004, 0), (65536, 16)):
+        flat = torch.from_numpy(rng.integers(0, 256, 9 * size + shift, dtype=np.uint8)).cuda()
+        buffers.append(flat[shift:].view(9, size))
+        want.append(buffers[-1].clone())
+    moves = [[3, 0], [-1, -1], [8, 5], [2, 9], [4, 4], [7, 1]]
+    ops.kv_cache_copy_pages(torch.tensor(moves, dtype=torch.int32, device="cuda"), buffers)
+    for got, w in zip(buffers, want):
+        for a, b in ((3, 0), (8, 5), (7, 1)):
+            w[b] = w[a]
+        assert torch.equal(got, w), got.shape
+
+
+def test_copy_pages_of_more_moves_than_workgroups():
+    moves = torch.full((3 << 20, 2), -1, dtype=torch.int32, device="cuda")
+    for at, pair in ((0, [1, 2]), ((1 << 21) + 3, [5, 0]), ((3 << 20) - 1, [4, 3])):
+        moves[at] = torch.tensor(pair, dtype=torch.int32)
+    large = torch.arange(6 * 5000, dtype=torch.int32, device="cuda").view(6, 5000)
+    small = torch.arange(6 * 8, dtype=torch.int32, device="cuda").view(6, 8)
+    want = [t[[5, 1, 1, 4, 4, 5]].clone() for t in (large, small)]
+    ops.kv_cache_copy_pages(moves, [large, small])
+    assert torch.equal(large, want[0]) and torch.equal(small, want[1])
+
+
 @pytest.mark.parametrize("kind", KINDS)
 def test_a_generation(kind):
     """Reserve, write, attend, fork, copy, diverge, free, compact, copy, attend again: against the plain calls at every
@@ -680,6 +709,67 @@ def test_calls_replay_from_a_graph():
         got = list(tensors[:4]) + [t for c in calls[1:] for t in c.result]
         for i, (g, w) in enumerate(zip(got, want)):
             assert torch.equal(g, w), (turn, i)
+
+
+@pytest.mark.parametrize("new", [[1, 2, 1], [80, 1, 3]])
+def test_graphs_that_share_scratch(new):
+    """Two graphs whose calls have one scratch between them, replayed in turn."""
+    rng = np.random.default_rng(79)
+    scratch = torch.empty(64 << 20, dtype=torch.uint8, device="cuda")
+    calls = []
+    for lens in ([500, 3000, 31], [90, 700, 2000]):
+        pool = Pool(rng, "s8", lens, 2, 64, 64, 16, width=50)
+        q, _ = bf16(rng.standard_normal((sum(new), 2 * 32, 64)))
+        calls.append(ops.kv_cache_attention(q, *pool.device(), dev(offsets(new)), lse=True, scratch=scratch, build_only=True))
+    want = []
+    for c in calls:
+        c.run()
+        want.append([t.clone() for t in c.result])
+    torch.cuda.synchronize()
+    graphs = []
+    side = torch.cuda.Stream()
+    for c in calls:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            c.run()
+    for turn in range(4):
+        for c in calls:
+            for t in c.result:
+                t.fill_(3)
+        scratch.fill_(0xff if turn % 2 else 0)
+        for g in graphs[::1 if turn % 2 else -1]:
+            g.replay()
+        torch.cuda.synchronize()
+        for c, w in zip(calls, want):
+            assert all(torch.equal(a, b) for a, b in zip(c.result, w))
+
+
+def test_calls_from_two_threads():
+    """Each thread with calls and a stream of its own."""
+    rng = np.random.default_rng(83)
+    work = []
+    for new, lens in (([1, 1], [900, 4000]), ([50, 1], [300, 1000])):
+        pool = Pool(rng, "f8", lens, 2, 64, 32, 8)
+        q, _ = bf16(rng.standard_normal((sum(new), 2 * 64, 64)))
+        call = ops.kv_cache_attention(q, *pool.device(), dev(offsets(new)), build_only=True)
+        want = call.run().clone()
+        work.append((call, want, []))
+    torch.cuda.synchronize()
+
+    def go(call, want, wrong):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                call.result.fill_(5)
+                call.run()
+                if not torch.equal(call.result, want):
+                    wrong.append(1)
+    threads = [threading.Thread(target=go, args=w) for w in work]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not any(w[2] for w in work)
 
 
 def test_calls_on_another_stream():

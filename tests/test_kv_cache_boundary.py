@@ -87,6 +87,13 @@ def test_attention_refuses():
     refused(t, frame(q=(BF16, None, (7, 6, 32))), "null q or out")
 
 
+def test_sizes_that_a_grid_cannot_hold():
+    c = cache()
+    q = (BF16, FAKE, ((1 << 22) + 1, 128, 32))
+    refused("xla_amd.kv_cache_attention", ffi.Frame(ffi.Host(), [q] + c, [q], {}), "2\\^29 rows times heads")
+    refused("xla_amd.kv_cache_write", write_frame(c, k=(BF16, FAKE, (1 << 24, 2, 32))), "fewer than 2\\^24 rows")
+
+
 def pages_frame(op="FREE", batch=3, width=5, pages=8, request=(S32, FAKE, (2,)), moves=0, status=2, page=16, scratch=1 << 20,
                 new=2 * FAKE, shapes=None):
     state = [(S32, FAKE, (batch, width)), (S32, FAKE, (batch,)), (S32, FAKE, (pages,))]
@@ -197,4 +204,8 @@ def test_scratch_sizes():
     L = ffi.library()
     assert L.xla_amd_kv_cache_pages_workspace_bytes(3, 8, 2) >= 3 * 8 * 4
     assert L.xla_amd_kv_cache_pages_workspace_bytes(-1, 8, 2) == 0
-    assert L.xla_amd_kv_cache_attention_workspace_bytes(0, 0, 8, 8, 128, 0) == 0
+    size = L.xla_amd_kv_cache_attention_workspace_bytes
+    assert size(0, 0, 8, 8, 128, 0) == 0
+    # the pieces are as many as the device takes at a time, however long the cache or the prompt
+    assert size(1, 1, 64, 8, 128, 1 << 24) <= 512 * 2 * 16 * (130 * 4 + 1)
+    assert size(1 << 16, 4, 64, 8, 128, 1 << 24) <= 512 * 2 * 32 * (130 * 4 + 1) + 1024 * 128 * (130 * 4 + 1)

@@ -39,7 +39,7 @@ int MakeKvCacheView(const XlaAmdKvCache& p, const char* what, KvCacheView* c) {
   if (p.kv_heads < 1 || p.kv_heads > 1024) return Fail(kBad, "%s: kv_heads must be 1 to 1024", what);
   if (p.pages > INT32_MAX || p.rows >= (1 << 24) || p.batch > (1 << 20) ||
       p.table_width > (int64_t)(INT32_MAX - 1024) / p.page_size)
-    return Fail(kBad, "%s: at most 2^31 - 1 pages, 2^24 - 1 rows, 2^20 sequences and 2^31 positions", what);
+    return Fail(kBad, "%s: at most 2^31 - 1 pages, fewer than 2^24 rows, 2^20 sequences and 2^31 positions", what);
   if (p.batch > 0 && p.rows > 0) {
     if (!p.kv_lens || !p.q_offsets || (p.table_width > 0 && !p.page_table))
       return Fail(kBad, "%s: null page_table, kv_lens or q_offsets", what);
