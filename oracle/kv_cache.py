@@ -59,17 +59,17 @@ def write(x, codes, scales, kind, page_table, kv_lens, q_offsets):
 
 def attention(q, k_codes, v_codes, k_scales, v_scales, kind, page_table, kv_lens, q_offsets, scale, causal=True, window=0,
               softcap=0.0):
-    """(out, lse, spread, slack) in 64 bits for q [rows, q_heads, head].  spread [rows, q_heads, head] is
+    """(out, lse, spread, slack, largest) in 64 bits for q [rows, q_heads, head].  spread [rows, q_heads, head] is
     sum_j w_j |v_j|, the size that errors of the weights act on; slack [rows, q_heads] bounds how far f32 sums
     of head products, in any order, leave a score: (head + 8) 2^-24 max_j sum_d |q_d k_jd| scale, and three
-    roundings of the score itself."""
+    roundings of the score itself; largest [rows, q_heads] is max_j w_j |scale of v_j|."""
     rows, q_heads, head = q.shape
     pages, heads, page, _ = k_codes.shape
     block = page // k_scales.shape[2]
     group = q_heads // heads
     out = np.zeros((rows, q_heads, head))
     spread, slack = np.zeros_like(out), np.zeros((rows, q_heads))
-    lse = np.full((rows, q_heads), -np.inf)
+    lse, largest = np.full((rows, q_heads), -np.inf), np.zeros((rows, q_heads))
     for b, (row0, n, length) in enumerate(sequences(rows, q_offsets, kv_lens, page_table.shape[1], page)):
         if n == 0 or length == 0:
             continue
@@ -90,6 +90,7 @@ def attention(q, k_codes, v_codes, k_scales, v_scales, kind, page_table, kv_lens
                 x = x * scales[pg, h, j % page // block].astype(np.float64)[:, None]
                 return np.where(any_row[:, None], x, 0.0)
             k, v = read(k_codes, k_scales), read(v_codes, v_scales)
+            vs = np.where(any_row, np.abs(v_scales[pg, h, j % page // block].astype(np.float64)), 0.0)
             for g in range(group):
                 qq = q[row0:row0 + n, h * group + g].astype(np.float64)
                 x = qq @ k.T * scale
@@ -109,18 +110,21 @@ def attention(q, k_codes, v_codes, k_scales, v_scales, kind, page_table, kv_lens
                 spread[at] = np.where(some[:, None], w @ np.abs(v) / safe, 0.0)
                 lse[at] = np.where(some, top + np.log(np.where(some, total, 1.0)), -np.inf)
                 slack[at] = np.where(seen, room, 0.0).max(1, initial=0.0)
-    return out, lse, spread, slack
+                largest[at] = np.where(some, (w * vs[None, :]).max(1, initial=0.0) / safe[:, 0], 0.0)
+    return out, lse, spread, slack, largest
 
 
-def attention_tolerance(out, lse, spread, slack, positions):
-    """Bounds on |out - exact| and |lse - exact| for a bf16 result of f32 sums whose weights are rounded to bf16:
-    half a bf16 step (2^-8) of the result, half a step of every weight; a weight is off by its score's slack
+def attention_tolerance(out, lse, spread, slack, largest, positions):
+    """Bounds on |out - exact| and |lse - exact| for a bf16 result of f32 sums whose weights times scales are rounded to
+    f16: half a bf16 step (2^-8) of the result, half an f16 step (2^-11) of every weight, or 2^-25 of the row's largest
+    where that is more (f16's smallest step is 2^-24, the largest is kept at 1 or above), times a code (up to 448) for
+    each of `positions`; a weight is off by its score's slack
     against the maximum's (2 slack) and by the exponential (2^-21); sums of `positions` weights by their
     number of 2^-24 roundings, in the numerator and in the denominator."""
     sums = (positions + 16) * 2.0 ** -24
     # above the formula's terms stands only their product, below 2^-8 of each: the factor 1.01
-    tol = 1.01 * (2.0 ** -8 * np.abs(out) + (2.0 ** -8 + 2.0 ** -20 + 2 * sums) * spread
-                  + 4 * slack[..., None] * spread) + 1e-37
+    tol = 1.01 * (2.0 ** -8 * np.abs(out) + (2.0 ** -11 + 2.0 ** -20 + 2 * sums) * spread
+                  + 4 * slack[..., None] * spread + positions * 448 * 2.0 ** -25 * largest[..., None]) + 1e-37
     fine = np.where(np.isfinite(lse), np.abs(lse), 0.0)
     return tol, 1.01 * (2 * slack + sums + 2.0 ** -20 + 2.0 ** -23 * fine)
 

@@ -62,9 +62,9 @@ def check_attention(pool, q, q_offsets, *, lse=True, scratch="auto", tiny=0.0, *
     scale = kw.pop("scale", q.shape[2] ** -0.5)
     out, got_lse = ops.kv_cache_attention(qt, *pool.device(), dev(q_offsets), scale=scale, lse=True, scratch=scratch, **kw)
     torch.cuda.synchronize()
-    ref, ref_lse, spread, slack = plain.attention(qf, pool.k, pool.v, pool.ks, pool.vs, pool.kind, pool.table, pool.lens,
+    ref, ref_lse, spread, slack, largest = plain.attention(qf, pool.k, pool.v, pool.ks, pool.vs, pool.kind, pool.table, pool.lens,
                                                   q_offsets, np.float32(scale), **kw)
-    tol, tol_lse = plain.attention_tolerance(ref, ref_lse, spread, slack, int(pool.lens.max(initial=0)))
+    tol, tol_lse = plain.attention_tolerance(ref, ref_lse, spread, slack, largest, int(pool.lens.max(initial=0)))
     got = out.float().cpu().numpy().astype(np.float64)
     bad = ~(np.abs(got - ref) <= tol + tiny)
     assert not bad.any(), (int(bad.sum()), bad.size, [(tuple(i), got[tuple(i)], ref[tuple(i)], tol[tuple(i)]) for i in np.argwhere(bad)[:4]])
@@ -184,6 +184,27 @@ def test_a_value_scale_that_is_no_number(kind, group, bad):
     assert ffi.last_kernel().startswith("kv_cache_attention_prompt") == (group == 64)
     assert torch.isnan(out[32:]).all() and torch.isnan(lse[32:]).all()
     assert torch.isfinite(out[:32]).all() and torch.isfinite(lse[:32]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads, new", [(2, 1), (64, 60)])
+@pytest.mark.parametrize("scale", [1e-4, 0.01, 300.0])
+def test_many_small_weights(kind, heads, new, scale):
+    """One position has all but 2% of the weight and values of 0; 20000 with 2^-20 each have the result.  Each of these
+    weights is rounded to f16 by at most 2^-25 of the largest one, 2^-5 of itself; they are alike, so it stays that much."""
+    n = 20000
+    pool = Pool(np.random.default_rng(3), kind, [n + new], 1, 64, 64, 16)
+    pool.k[:], pool.v[:] = 0, (64 if kind == "s8" else 0x68)      # 64 in f8e4m3fn
+    pool.k[pool.table[0, 0], 0, 7] = 1 if kind == "s8" else 0x38   # 1
+    pool.v[pool.table[0, 0], 0, 7] = 0
+    pool.ks[:], pool.vs[:] = 1.0, scale
+    q = np.zeros((new, heads, 64))
+    q[:, :, 0] = 14.0
+    out = ops.kv_cache_attention(bf16(q)[0], *pool.device(), dev(offsets([new])), causal=False, scale=20 * np.log(2.0) / 14)
+    w = 2.0 ** -20 * (n + new - 1)
+    want = 64 * scale * w / (1 + w)
+    got = out.float().cpu().numpy()
+    assert (np.abs(got / want - 1) <= 2.0 ** -5 + 2.0 ** -8 + 1e-4).all(), (got.min(), got.max(), want)
 
 
 @pytest.mark.parametrize("kind", KINDS)

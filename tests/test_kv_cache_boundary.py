@@ -175,12 +175,12 @@ def test_plain_attention_by_hand():
     one = np.ones((1, 1, 16), np.float32)
     q = np.zeros((2, 1, 16), np.float32)
     q[:, 0, 0] = np.log(3.0)
-    out, lse, _, _ = plain.attention(q, k, v, one, one, "s8", np.array([[0]]), [2], [0, 2], 1.0)
+    out, lse = plain.attention(q, k, v, one, one, "s8", np.array([[0]]), [2], [0, 2], 1.0)[:2]
     assert np.allclose(out[:, 0, 0], [10.0, 12.5])      # weights 1, then 3/4 and 1/4
     assert np.allclose(lse[:, 0], [np.log(3.0), np.log(4.0)])
-    out, lse, _, _ = plain.attention(q, k, v, one, one, "s8", np.array([[0]]), [2], [0, 2], 1.0, window=1)
+    out, lse = plain.attention(q, k, v, one, one, "s8", np.array([[0]]), [2], [0, 2], 1.0, window=1)[:2]
     assert np.allclose(out[:, 0, 0], [10.0, 20.0])
-    out, lse, _, _ = plain.attention(q, k, v, one, one, "s8", np.array([[-1]]), [2], [0, 2], 1.0)
+    out, lse = plain.attention(q, k, v, one, one, "s8", np.array([[-1]]), [2], [0, 2], 1.0)[:2]
     assert not out.any() and np.isneginf(lse).all()
 
 

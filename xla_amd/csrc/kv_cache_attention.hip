@@ -43,7 +43,7 @@ struct __attribute__((aligned(16))) CutTile {
 //                 values d = c DP/16 .. of those eight keys, transposed in registers while they are widened.
 // The sums over d and over keys run in whatever order the operands share, so nothing is shuffled but maxima.
 // Scales stay out of the operands: the key's on the f32 score, the value's on the weight, which is rounded to
-// bf16 there (2^-9 of each weight, where the result is rounded by as much; f32 sums).
+// f16 there.
 //
 // Where the keys are split: all sequences' units (times their tiles of rows) stand in one line, which is cut
 // into as many equal pieces as there are workers for a head, so a batch of mixed lengths fills the device
@@ -51,7 +51,9 @@ struct __attribute__((aligned(16))) CutTile {
 // scratch, at most two for each worker, and a second launch joins them in order.  The worker in whose range a cut
 // tile begins notes where its pieces are, so the second launch looks for nothing.
 //
-// Bound: HBM, 2 (head + 4 / block) bytes for each position and cache head.
+// Bound: HBM, 2 (head + 4 / block) bytes for each position and cache head.  64 sequences of up to 8192 positions, 8 heads
+// of 128: 110 us, 4.9 TB/s, where 512 workgroups that read pages of 64 KB in any order reach 6.1 and a linear read 7.05;
+// four sequences of 131072: 186 us, 5.3 TB/s.  The same call on pages that stay in the caches takes 75 to 79 us.
 constexpr int kUnit = 128;
 
 struct DecodeView {
@@ -161,28 +163,89 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t lo, uint32_t hi) {
   return __builtin_bit_cast(bf16x8, uintx4{widen2<F8, 0>(lo), widen2<F8, 2>(lo), widen2<F8, 0>(hi), widen2<F8, 2>(hi)});
 }
 
-// Bytes T and T + 1 (T even; word T / 4) of eight keys -> eight bf16 each.
+typedef _Float16 halfx2 __attribute__((ext_vector_type(2)));
+typedef _Float16 halfx8 __attribute__((ext_vector_type(8)));
+
+// Two codes at bytes 0 and 2 (S8; the other bytes 0) -> two f16, exact: 1024 + 128 + c, less 1152.
+__device__ __forceinline__ uint32_t s8_to_f16(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_bit_cast(halfx2, w ^ 0x64806480u) - halfx2{(_Float16)1152.0f, (_Float16)1152.0f});
+}
+
+// Four codes -> four f16, exact.
+template <bool F8>
+__device__ __forceinline__ uintx2 widen4_f16(uint32_t w) {
+  if constexpr (F8) {
+    return uintx2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, false)),
+                  __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, true))};
+  } else {
+    return uintx2{s8_to_f16(__builtin_amdgcn_perm(0u, w, 0x0c010c00u)), s8_to_f16(__builtin_amdgcn_perm(0u, w, 0x0c030c02u))};
+  }
+}
+
+template <bool F8>
+__device__ __forceinline__ halfx8 widen8_f16(uint32_t lo, uint32_t hi) {
+  const uintx2 a = widen4_f16<F8>(lo), b = widen4_f16<F8>(hi);
+  return __builtin_bit_cast(halfx8, uintx4{a[0], a[1], b[0], b[1]});
+}
+
+// Bytes T and T + 1 (T even; word T / 4) of eight keys -> eight f16 each.
 template <bool F8, int T, int N>
-__device__ __forceinline__ void columns(const uint32_t (&k)[8][N], bf16x8& first, bf16x8& second) {
-  constexpr int W = T >> 2, I = T & 3;
-  uintx4 r, t;
+__device__ __forceinline__ void columns(const uint32_t (&k)[8][N], uintx4& first, uintx4& second) {
+  constexpr int W = T >> 2;
+  constexpr uint32_t I = T & 3;
 #pragma unroll
   for (int p = 0; p < 4; ++p) {
     const uint32_t a = k[2 * p][W], b = k[2 * p + 1][W];
     if constexpr (F8) {
       // byte I of both keys, then byte I + 1 of both, as the conversion reads them
-      const uint32_t pairs = __builtin_amdgcn_perm(b, a, 0x05010400u + 0x01010101u * I);
-      r[p] = widen2<true, 0>(pairs);
-      t[p] = widen2<true, 2>(pairs);
+      const uintx2 both = widen4_f16<true>(__builtin_amdgcn_perm(b, a, 0x05010400u + 0x01010101u * I));
+      first[p] = both[0];
+      second[p] = both[1];
     } else {
-      const float x = (float)(int8_t)(a >> (8 * I)), y = (float)(int8_t)(b >> (8 * I));
-      const float z = (float)(int8_t)(a >> (8 * I + 8)), w = (float)(int8_t)(b >> (8 * I + 8));
-      r[p] = __builtin_amdgcn_perm(f32_to_bits(y), f32_to_bits(x), 0x07060302u);
-      t[p] = __builtin_amdgcn_perm(f32_to_bits(w), f32_to_bits(z), 0x07060302u);
+      first[p] = s8_to_f16(__builtin_amdgcn_perm(b, a, 0x0c040c00u + 0x00010001u * I));
+      second[p] = s8_to_f16(__builtin_amdgcn_perm(b, a, 0x0c050c01u + 0x00010001u * I));
     }
   }
-  first = __builtin_bit_cast(bf16x8, r);
-  second = __builtin_bit_cast(bf16x8, t);
+}
+
+// A weight times its value's scale goes into the matrix instruction as f16, which rounds it by 2^-11 at most; bf16 would
+// by 2^-8, as much as the result's own rounding, and the result would be 1.4 times as far from the exact one.  f16's range
+// is narrow, so a row's weights and sums carry a factor, a power of two, that keeps every scale times the factor in
+// [kLeast, kMost].  Weights are 2^8 at most (the maximum in use may lag behind by that much), so none passes 2^15, and
+// next to a row's largest one the others keep an absolute error of 2^-25 of it.  Where a scale leaves that range, the
+// weights themselves and their sum so far (`weighed`, with the factor) choose the next factor, in a branch.
+constexpr float kMost = 128.0f, kLeast = 1.0f, kLag = 8.0f;
+
+// of scales times the factor
+template <int N>
+__device__ __forceinline__ bool factor_fits(const float (&x)[N]) {
+  float most = __builtin_fabsf(x[0]), least = most;
+#pragma unroll
+  for (int i = 1; i < N; ++i) {
+    most = __builtin_fmaxf(most, __builtin_fabsf(x[i]));
+    least = __builtin_fminf(least, __builtin_fabsf(x[i]));
+  }
+  return least >= kLeast && most <= kMost;
+}
+
+// A factor is 2^-125 to 2^100, the step from one to the next at most 2^100 up.
+__device__ __forceinline__ float reciprocal(float factor) { return bits_to_f32((254u << 23) - f32_to_bits(factor)); }
+
+// The factor for a row whose largest weight times scale is `most`, if not 0: their product is 32 to 64.
+__device__ __forceinline__ float new_factor(float most, float factor) {
+  const uint32_t e = min(max(f32_to_bits(most) >> 23, 32u), 254u);
+  const float now = __builtin_fminf(bits_to_f32((259u - e) << 23), factor * 0x1p100f);
+  return most > 0.0f ? now : factor;
+}
+
+// A scale times a new factor; finite, so that a weight of 0 cancels it.
+__device__ __forceinline__ float finite_product(float scale, float factor) {
+  constexpr float kMax = 3.4028234663852886e38f;
+  return __builtin_amdgcn_fmed3f(scale * factor, -kMax, kMax);
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(floatx2{a, b}, halfx2));
 }
 
 // Keeps what follows in its branch: work that few steps need is not done by all of them and thrown away.
@@ -412,10 +475,12 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
     }
 
     floatx4 acc[QT][VT];
-    float top[QT], sum[QT];
+    float top[QT], sum[QT], factor_v[QT], weighed[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
       top[t] = -1e30f;  // below every score, and finite
+      factor_v[t] = 1.0f;
+      weighed[t] = 0.0f;
       sum[t] = 0.0f;
 #pragma unroll
       for (int i = 0; i < VT; ++i) acc[t][i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -428,7 +493,7 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
       const uint8_t* const from = mine + slot * SLOT;
       uintx4 k[2][NI];
       intx2 raw[VT];
-      float ks[2][S], vs[2][S];
+      float ks[2 * S], vs[2 * S];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -437,8 +502,8 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int i = 0; i < S; ++i) {
-          ks[h][i] = *reinterpret_cast<const float*>(from + 64 * DP + 4 * (16 * h + 4 * grp + i));
-          vs[h][i] = *reinterpret_cast<const float*>(from + 64 * DP + 4 * (32 + 16 * h + 4 * grp + i));
+          ks[h * S + i] = *reinterpret_cast<const float*>(from + 64 * DP + 4 * (16 * h + 4 * grp + i));
+          vs[h * S + i] = *reinterpret_cast<const float*>(from + 64 * DP + 4 * (32 + 16 * h + 4 * grp + i));
         }
 #pragma unroll
       for (int t = 0; t < VT; ++t) raw[t] = read_columns(from + (vread ^ (t << 4)));
@@ -465,9 +530,7 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
         for (int t = 0; t < VT; ++t) raw[t] = intx2{(int)(raw[t][0] & keep[0]), (int)(raw[t][1] & keep[1])};
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < S; ++i) keep_to_its_rows(ks[h][i], vs[h][i]);
+      for (int i = 0; i < 2 * S; ++i) keep_to_its_rows(ks[i], vs[i]);
       floatx4 s[QT][2];
 #pragma unroll
       for (int t = 0; t < QT; ++t)
@@ -483,12 +546,12 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
           // one piece widened while the one before is multiplied, and no more of them in registers
           __builtin_amdgcn_sched_barrier(0);
         }
-      bf16x8 p[QT];
+      halfx8 p[QT];
 #pragma unroll
       for (int t = 0; t < QT; ++t) {
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = s[t][e >> 2][e & 3] * (ks[e >> 2][SMALL ? (e & 3) : 0] * factor);
+        for (int e = 0; e < 8; ++e) y[e] = s[t][e >> 2][e & 3] * (ks[(e >> 2) * S + (e & (S - 1))] * factor);
         if (cap > 0.0f) {
           KV_CACHE_RARE();
 #pragma unroll
@@ -506,32 +569,60 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
         float most = y[0];
 #pragma unroll
         for (int e = 1; e < 8; ++e) most = __builtin_fmaxf(most, y[e]);
-        // the maximum in use may lag behind by up to 2^8, which f32 and bf16 weights bear
-        if (__any(most > top[t] + 8.0f)) {
+        if (__any(most > top[t] + kLag)) {
           most = __builtin_fmaxf(most, __shfl_xor(most, 16));
           most = __builtin_fmaxf(most, __shfl_xor(most, 32));
           const float now = __builtin_fmaxf(top[t], most);
           const float scale = __builtin_amdgcn_exp2f(top[t] - now);
           top[t] = now;
           sum[t] *= scale;
+          weighed[t] *= scale;
 #pragma unroll
           for (int i = 0; i < VT; ++i) acc[t][i] *= scale;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = __builtin_amdgcn_exp2f(y[e] - top[t]);
+        float x[2 * S];
+#pragma unroll
+        for (int i = 0; i < 2 * S; ++i) x[i] = vs[i] * factor_v[t];
+        if (__any(!factor_fits(x))) {
+          KV_CACHE_RARE();
+          float weight = weighed[t] * reciprocal(factor_v[t]);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) weight = __builtin_fmaxf(weight, __builtin_fabsf(y[e] * vs[(e >> 2) * S + (e & (S - 1))]));
+          weight = __builtin_fmaxf(weight, __shfl_xor(weight, 16));
+          weight = __builtin_fmaxf(weight, __shfl_xor(weight, 32));
+          const float now = new_factor(weight, factor_v[t]);
+          const float step = now * reciprocal(factor_v[t]);
+          factor_v[t] = now;
+          weighed[t] *= step;
+#pragma unroll
+          for (int i = 0; i < VT; ++i) acc[t][i] *= step;
+#pragma unroll
+          for (int i = 0; i < 2 * S; ++i) x[i] = finite_product(vs[i], now);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float four = (y[4 * h] + y[4 * h + 1]) + (y[4 * h + 2] + y[4 * h + 3]);
+          sum[t] += four;
+          if constexpr (SMALL) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) weighed[t] = __builtin_fmaf(y[4 * h + e], __builtin_fabsf(x[4 * h + e]), weighed[t]);
+          } else {
+            weighed[t] = __builtin_fmaf(four, __builtin_fabsf(x[h]), weighed[t]);
+          }
+        }
         uintx4 w;
 #pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const int h = e >> 2;
-          const float p0 = __builtin_amdgcn_exp2f(y[e] - top[t]), p1 = __builtin_amdgcn_exp2f(y[e + 1] - top[t]);
-          sum[t] += p0 + p1;
-          w[e >> 1] = pack_bf16x2(p0 * vs[h][SMALL ? (e & 3) : 0], p1 * vs[h][SMALL ? (e & 3) + 1 : 0]);
-        }
-        p[t] = __builtin_bit_cast(bf16x8, w);
+        for (int e = 0; e < 8; e += 2)
+          w[e >> 1] = pack_f16x2(y[e] * x[(e >> 2) * S + (e & (S - 1))], y[e + 1] * x[(e >> 2) * S + ((e + 1) & (S - 1))]);
+        p[t] = __builtin_bit_cast(halfx8, w);
       }
 #pragma unroll
       for (int i = 0; i < VT; ++i) {
-        const bf16x8 vv = widen8<F8>(raw[i][0], raw[i][1]);
+        const halfx8 vv = widen8_f16<F8>(raw[i][0], raw[i][1]);
 #pragma unroll
-        for (int t = 0; t < QT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vv, p[t], acc[t][i], 0, 0, 0);
+        for (int t = 0; t < QT; ++t) acc[t][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vv, p[t], acc[t][i], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -569,9 +660,10 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
         const int r = 16 * t + col;
         const float m = __builtin_fmaxf(__builtin_fmaxf(tops[0][r], tops[1][r]), __builtin_fmaxf(tops[2][r], tops[3][r]));
         const float scale = __builtin_amdgcn_exp2f(top[t] - m);
+        const float less = reciprocal(factor_v[t]);
 #pragma unroll
         for (int i = 0; i < VT; ++i)
-          *reinterpret_cast<floatx4*>(&sums[(wave * 16 + col) * NF + 16 * i + 4 * grp]) = acc[t][i] * scale;
+          *reinterpret_cast<floatx4*>(&sums[(wave * 16 + col) * NF + 16 * i + 4 * grp]) = acc[t][i] * scale * less;
       }
       __syncthreads();
       const int r = 16 * t + (tid >> 4);
@@ -627,9 +719,9 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
 // 16-byte pieces of a key row are stored at piece ^ (position & 15), those of a value row at
 // piece ^ ((d ^ d >> 2) & 7): eight lanes that read or write together then meet eight different places.
 //
-// Bound: two waves share a SIMD, and each needs 1312 cycles of vector instructions (a quarter of them exponentials) and
+// Bound: two waves share a SIMD, and each needs 1400 cycles of vector instructions (a quarter of them exponentials) and
 // 1024 of matrix instructions for a stage of a head of 128, the matrix pipes being busy for 38% of the time.  8192 rows of
-// 32 heads on 8192 positions, causal: 601 us, 915 TFLOP/s, where a large product of matrices reaches 1357.
+// 32 heads on 8192 positions, causal: 635 us, 866 TFLOP/s, where a large product of matrices reaches 1357.
 constexpr int kStage = 64;
 constexpr int kPromptRows = 128;
 // Where a call has few tiles, their positions are cut: into pieces that give kPieces workgroups at most (six chunks of
@@ -713,7 +805,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     sees_lo = v.a.window > 0 ? max(0, p - v.a.window + 1) : 0;
   }
   floatx16 acc[DP / 32];
-  float top = -1e30f, sum = 0.0f;
+  float top = -1e30f, sum = 0.0f, factor_v = 1.0f, weighed = 0.0f;
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -792,23 +884,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
       uint32_t one[8][1];
 #pragma unroll
       for (int e = 0; e < 8; ++e) one[e][0] = vraw[I][e];
-      bf16x8 va, vb;
+      uintx4 va, vb;
       columns<F8, T>(one, va, vb);
-      vals[buf][d * 8 + ((2 * wave + vhalf) ^ ((d ^ (d >> 2)) & 7))] = __builtin_bit_cast(uintx4, va);
-      vals[buf][d * 8 + 8 + ((2 * wave + vhalf) ^ (((d + 1) ^ (d >> 2)) & 7))] = __builtin_bit_cast(uintx4, vb);
+      vals[buf][d * 8 + ((2 * wave + vhalf) ^ ((d ^ (d >> 2)) & 7))] = va;
+      vals[buf][d * 8 + 8 + ((2 * wave + vhalf) ^ (((d + 1) ^ (d >> 2)) & 7))] = vb;
     }
   };
 
   floatx16 sc[2];
-  bf16x8 p[2][2];
-  float kq[4 * S], vq[4 * S], more;
+  halfx8 p[2][2];
+  float kq[4 * S], vq[4 * S], more, more_weighed;  // vq: with the factor
   auto key_piece = [&](int buf, int kt, int k) KV_CACHE_INLINE {
     const int pos = 32 * kt + n;
     return __builtin_bit_cast(bf16x8, keys[buf][pos * KC + ((2 * k + h) ^ (pos & KX))]);
   };
   auto value_piece = [&](int buf, int kt, int at) KV_CACHE_INLINE {  // at: which 16 positions, then which 32 values
     const int g = 2 * kt + at / (DP / 32), d = 32 * (at % (DP / 32)) + n;
-    return __builtin_bit_cast(bf16x8, vals[buf][d * 8 + ((2 * g + h) ^ ((d ^ (d >> 2)) & 7))]);
+    return __builtin_bit_cast(halfx8, vals[buf][d * 8 + ((2 * g + h) ^ ((d ^ (d >> 2)) & 7))]);
   };
   auto score = [&](auto kt_, bf16x8 a, auto k_) KV_CACHE_INLINE {
     constexpr int KT = decltype(kt_)::value, K = decltype(k_)::value;
@@ -819,9 +911,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     }
     sc[KT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, q[K], from, 0, 0, 0);
   };
-  auto result = [&](auto kt_, bf16x8 a, auto at_) KV_CACHE_INLINE {
+  auto result = [&](auto kt_, halfx8 a, auto at_) KV_CACHE_INLINE {
     constexpr int KT = decltype(kt_)::value, G = decltype(at_)::value / (DP / 32), I = decltype(at_)::value % (DP / 32);
-    acc[I] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, p[KT][G], acc[I], 0, 0, 0);
+    acc[I] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, p[KT][G], acc[I], 0, 0, 0);
   };
   // The scales of a half; where scores are capped or some position is not seen, the scores themselves are made final.
   auto prepare = [&](bool edge, int buf, int j0, auto kt_) KV_CACHE_INLINE {
@@ -830,7 +922,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     for (int i = 0; i < 4 * S; ++i) {
       const int pos = 32 * KT + 8 * (i / S) + 4 * h + i % S;
       kq[i] = kscale[buf][pos];
-      vq[i] = vscale[buf][pos];
+      vq[i] = vscale[buf][pos] * factor_v;
     }
     if (cap > 0.0f) {
       KV_CACHE_RARE();
@@ -862,18 +954,23 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     for (int e = 0; e < 4; ++e) w[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[KT][4 * I + e], kq[I * S + (e & (S - 1))], -top));
     const float four = (w[0] + w[1]) + (w[2] + w[3]);
     more = I == 0 ? four : more + four;
+    if constexpr (I == 0) more_weighed = 0.0f;
+    if constexpr (!SMALL) more_weighed = __builtin_fmaf(four, __builtin_fabsf(vq[I]), more_weighed);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] *= vq[I * S + (e & (S - 1))];
+    for (int e = 0; e < 4; ++e) {
+      w[e] *= vq[I * S + (e & (S - 1))];
+      if constexpr (SMALL) more_weighed += __builtin_fabsf(w[e]);
+    }
     uintx4 packed = I & 1 ? __builtin_bit_cast(uintx4, p[KT][I >> 1]) : uintx4{0u, 0u, 0u, 0u};
-    packed[2 * (I & 1)] = pack_bf16x2(w[0], w[1]);
-    packed[2 * (I & 1) + 1] = pack_bf16x2(w[2], w[3]);
-    p[KT][I >> 1] = __builtin_bit_cast(bf16x8, packed);
+    packed[2 * (I & 1)] = pack_f16x2(w[0], w[1]);
+    packed[2 * (I & 1) + 1] = pack_f16x2(w[2], w[3]);
+    p[KT][I >> 1] = __builtin_bit_cast(halfx8, packed);
   };
-  // The maximum in use may lag behind by up to 2^10, which f32 and bf16 weights bear; where the weights' sum shows
-  // more, the half is weighed again.
-  auto catch_up = [&](auto kt_) KV_CACHE_INLINE {
+  // Where the weights' sum shows that the maximum in use lags too far behind, or a scale leaves the factor's range, the
+  // half is weighed again.
+  auto catch_up = [&](int buf, auto kt_) KV_CACHE_INLINE {
     constexpr int KT = decltype(kt_)::value;
-    if (__any(more > 1024.0f)) {
+    if (__any(more > 256.0f || !factor_fits(vq))) {
       KV_CACHE_RARE();
       float most = -INFINITY;
 #pragma unroll
@@ -883,11 +980,27 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
       const float scale = __builtin_amdgcn_exp2f(top - now);
       top = now;
       sum *= scale;
+      float weight = weighed * scale * reciprocal(factor_v);
 #pragma unroll
-      for (int i = 0; i < DP / 32; ++i) acc[i] *= scale;
+      for (int i = 0; i < 4 * S; ++i) vq[i] = vscale[buf][32 * KT + 8 * (i / S) + 4 * h + i % S];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = (r >> 2) * S + (r & (S - 1));
+        weight = __builtin_fmaxf(weight, __builtin_fabsf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[KT][r], kq[i], -top)) * vq[i]));
+      }
+      weight = __builtin_fmaxf(weight, __shfl_xor(weight, 32));
+      const float next = new_factor(weight, factor_v);
+      const float step = scale * (next * reciprocal(factor_v));
+      factor_v = next;
+      weighed *= step;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) acc[i] *= step;
+#pragma unroll
+      for (int i = 0; i < 4 * S; ++i) vq[i] = finite_product(vq[i], next);
       static_for<0, 4>([&](auto unit) KV_CACHE_INLINE { weigh(kt_, unit); });
     }
     sum += more;
+    weighed += more_weighed;
   };
   constexpr std::integral_constant<int, 0> kFirst{};
   constexpr std::integral_constant<int, 1> kSecond{};
@@ -924,27 +1037,27 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
           KV_CACHE_FENCE();
         });
       }
-      catch_up(kFirst);
+      catch_up(buf, kFirst);
       prepare(edge, buf, j0, kSecond);
       {
-        bf16x8 a = value_piece(buf, 0, 0);
+        halfx8 a = value_piece(buf, 0, 0);
         static_for<0, QK>([&](auto k) KV_CACHE_INLINE {
           constexpr int K = decltype(k)::value;
-          const bf16x8 now = a;
+          const halfx8 now = a;
           if constexpr (K + 1 < QK) a = value_piece(buf, 0, K + 1);
           result(kFirst, now, k);
           static_for<K * 4 / QK, (K + 1) * 4 / QK>([&](auto unit) KV_CACHE_INLINE { weigh(kSecond, unit); });
           KV_CACHE_FENCE();
         });
       }
-      catch_up(kSecond);
+      catch_up(buf, kSecond);
       // past the last stage, of whatever is there
       stage_scales(u + 1, buf ^ 1);
       {
-        bf16x8 a = value_piece(buf, 1, 0);
+        halfx8 a = value_piece(buf, 1, 0);
         static_for<0, QK>([&](auto k) KV_CACHE_INLINE {
           constexpr int K = decltype(k)::value;
-          const bf16x8 now = a;
+          const halfx8 now = a;
           if constexpr (K + 1 < QK) a = value_piece(buf, 1, K + 1);
           result(kSecond, now, k);
           static_for<K * PIECES / QK, (K + 1) * PIECES / QK>([&](auto at) KV_CACHE_INLINE { stage_piece(at, buf ^ 1); });
@@ -965,13 +1078,16 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   const bool joined = splits > 1;
   float* part = joined ? v.partial + ((int64_t)slot * c.heads + head) * RT * (c.head + 2) : nullptr;
   const float inverse = l == 0.0f ? 0.0f : 1.0f / l;
+  const float less = reciprocal(factor_v);
 #pragma unroll
   for (int i2 = 0; i2 < DP / 32; ++i2)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = 32 * i2 + 8 * e + 4 * h;
       if (d >= c.head) continue;
-      const floatx4 o = {acc[i2][4 * e], acc[i2][4 * e + 1], acc[i2][4 * e + 2], acc[i2][4 * e + 3]};
+      floatx4 o;
+#pragma unroll
+      for (int f = 0; f < 4; ++f) o[f] = acc[i2][4 * e + f] * less;
       if (joined) *reinterpret_cast<floatx4*>(part + (int64_t)r * c.head + d) = o;
       else *reinterpret_cast<uintx2*>(v.a.out + at_row * c.head + d) =
           uintx2{pack_bf16x2(o[0] * inverse, o[1] * inverse), pack_bf16x2(o[2] * inverse, o[3] * inverse)};
