@@ -1193,10 +1193,13 @@ DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_h
   if (few && d.tiles > most) d.tiles = most;
   const int64_t units = d.tiles * ((positions + kUnit - 1) / kUnit);
   const int64_t slots = 256 * decode_residents(d.dp);
-  int64_t w = (slots + kv_heads - 1) / kv_heads;
+  int64_t w = slots / kv_heads;  // no more than run at a time: each has an equal piece
   if (w > units) w = units;
   d.workers = w < 1 ? 1 : (int)w;
-  d.split = positions > kUnit && batch > 0;
+  // A second launch costs more than four units one after the other (two of a head above 128).  Eight heads of 128, cut and
+  // whole: one sequence of 500 positions 10.4 and 10.1 us, of 760 11.0 and 12.3; eight 12.3 and 10.5, 12.9 and 16.0;
+  // 64 of 500 19.8 and 17.9.  A head of 256: one of 250 12.9 and 11.0, of 500 12.9 and 14.9.
+  d.split = positions > (d.dp == 256 ? 2 : 4) * kUnit && batch > 0;
   d.bytes = d.split ? (size_t)(d.workers * (sizeof(CutTile) + kv_heads * 2 * 16 * d.qt * (head + 2) * 4)) : 0;
   return d;
 }
@@ -1288,7 +1291,8 @@ int LaunchKvCacheAttention(const XlaAmdKvCacheAttention& p, hipStream_t stream) 
   const int64_t positions = p.cache.table_width * p.cache.page_size;
   v.window = p.window >= positions ? 0 : (int)p.window;  // every position that a causal row sees is nearer
   const PromptPlan pr = PlanPrompt(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, positions);
-  const DecodePlan d = PlanDecode(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, positions, pr.used);
+  const int64_t reach = v.window > 0 ? min(positions, (int64_t)v.window + kUnit) : positions;  // of a row, in whole units
+  const DecodePlan d = PlanDecode(v.c.rows, v.c.batch, p.q_heads, p.cache.kv_heads, p.cache.head_size, reach, pr.used);
   DecodeView dv{};
   dv.a = v;
   dv.workers = d.workers;
