@@ -156,8 +156,8 @@ XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_rowwise_quantize_fp8(XLA_FFI_CallFrame* ca
  *   args: k, v BF16 [rows, kv_heads, head]; k_cache, v_cache; k_scales, v_scales; page_table S32 [batch, width];
  *         kv_lens S32 [batch] (with the new rows); q_offsets S32 [batch + 1]
  *   rets: k_cache, v_cache, k_scales, v_scales, the operands' own buffers (output_to_operand_aliasing)
- *   No two positions that a call writes may lie in one page row, and no block that it touches may belong to
- *   two sequences (XLA_AMD_TARGET_KV_CACHE_PAGES never shares a page that is not full).
+ *   Keys and values have buffers of their own.  No two positions that a call writes may lie in one page row, and no
+ *   block that it touches may belong to two sequences (XLA_AMD_TARGET_KV_CACHE_PAGES never shares a page that is not full).
  */
 XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_kv_cache_write(XLA_FFI_CallFrame* call_frame);
 

@@ -87,6 +87,10 @@ def test_attention_refuses():
     refused(t, frame(q=(BF16, None, (7, 6, 32))), "null q or out")
 
 
+def test_keys_and_values_in_one_buffer():
+    refused("xla_amd.kv_cache_write", write_frame(cache()), "buffers of their own")
+
+
 def test_sizes_that_a_grid_cannot_hold():
     c = cache()
     q = (BF16, FAKE, ((1 << 22) + 1, 128, 32))
@@ -144,6 +148,8 @@ def test_python_wrappers_refuse_what_a_frame_cannot_say():
         ops._operand(t[0], "k_cache", ops._CACHE, 4)
     with pytest.raises(TypeError, match="element type torch.int16"):
         ops._operand(t.to(torch.int16), "k_cache", ops._CACHE, 4)
+    with pytest.raises(TypeError, match="scratch: element type torch.float32"):
+        ops._operand(torch.zeros(4), "scratch", {torch.uint8: U8, torch.int8: S8}, 1)
     with pytest.raises(ValueError, match="op must be RESERVE"):
         ops.kv_cache_pages("reserve", None, None, None, page_size=16)
 

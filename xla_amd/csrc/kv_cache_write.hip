@@ -262,6 +262,8 @@ int LaunchKvCacheWrite(const XlaAmdKvCacheWrite& p, hipStream_t stream) {
   if ((((uintptr_t)p.k | (uintptr_t)p.v) & 15) != 0)
     return Fail(XLA_FFI_Error_Code_INVALID_ARGUMENT, "kv_cache_write: k and v must be aligned to 16 bytes");
   if (c.rows == 0 || c.batch == 0 || c.pages == 0 || c.width == 0) return 0;
+  if (c.codes[0] == c.codes[1] || c.scales[0] == c.scales[1])
+    return Fail(XLA_FFI_Error_Code_INVALID_ARGUMENT, "kv_cache_write: keys and values need buffers of their own");
   // n rows touch at most n blocks and at most (n - 2) / block + 2
   int64_t items = ((int64_t)c.rows >> c.block_log2) + 2 * (int64_t)c.batch;
   if (items > c.rows) items = c.rows;

@@ -279,9 +279,11 @@ def kv_cache_attention(q, k_cache, v_cache, k_scales, v_scales, page_table, kv_l
     q_heads is a multiple of kv_heads.  Row i of a sequence's n rows stands at position kv_lens[b] - n + i; it
     sees the positions below kv_lens[b], up to its own if causal, and the last `window` of those if window > 0.
     scale: softmax scale (default head ** -0.5); softcap c > 0: scores become c * tanh(score / c).
-    Rows that see nothing, or belong to no sequence, are 0 and their lse -inf."""
+    Rows that see nothing, or belong to no sequence, are 0 and their lse -inf.
+    scratch: bytes for sequences that several workgroups share, of any content; "auto" allocates them, None does without."""
     cache = (k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets)
-    device = _one_device(q, out, *cache)
+    given = None if scratch is None or isinstance(scratch, str) else scratch
+    device = _one_device(q, out, given, *cache)
     bf16 = {torch.bfloat16: dtypes.BF16}
     args = [_operand(q, "q", bf16, 3)] + _cache_operands(*cache)
     if out is None:
@@ -295,7 +297,7 @@ def kv_cache_attention(q, k_cache, v_cache, k_scales, v_scales, page_table, kv_l
             q.shape[0], kv_lens.shape[0], q.shape[1], k_cache.shape[1], q.shape[2],
             page_table.shape[1] * k_cache.shape[2]), device)
     if scratch is not None:
-        rets.append((dtypes.U8, scratch.data_ptr(), [scratch.numel()]))
+        rets.append(_operand(scratch, "scratch", {torch.uint8: dtypes.U8, torch.int8: dtypes.S8}, 1))
     attrs = {"causal": ffi.Attr.pred(causal), "window": ffi.Attr.i64(window), "softcap": ffi.Attr.f32(softcap)}
     if scale is not None:
         attrs["softmax_scale"] = ffi.Attr.f32(scale)
