@@ -725,9 +725,12 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
 constexpr int kStage = 64;
 constexpr int kPromptRows = 128;
 // Where a call has few tiles, their positions are cut: into pieces that give kPieces workgroups at most (six chunks of
-// prompts, 312 tiles and heads: 111 us uncut, 94 with 1024, 103 with 2048, 123 with 4096), kMostSplits for a tile, of
-// kLeastStages stages or more.  How many tiles there are is device data, so each workgroup counts them.
+// prompts, 312 tiles and heads: 82 us with 512, which cuts none, 73 with 768, 67 with 1024, 83 with 1536), kLeastSplits to
+// kMostSplits for a tile, of kLeastStages stages or more.  512 workgroups run at a time, so tiles that fill them once
+// stay whole: 4 chunks of 512 rows on 4096 positions (512 tiles and heads) take 199 us whole and 232 cut in two, two
+// prompts of 1024 64 and 79.  How many tiles there are is device data, so each workgroup counts them.
 constexpr int kPieces = 1024;
+constexpr int kLeastSplits = 3;
 constexpr int kMostSplits = 16;
 constexpr int kLeastStages = 4;
 
@@ -767,7 +770,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   const LineSpot spot = line_find(
       c.batch, lane, [&](int b) { return (int64_t)prompt_tiles(v.a, v.rows_from, b); },
       [&](int64_t total) {
-        if (v.partial && 2 * total <= v.pieces) splits = (int)min((uint32_t)v.pieces / max((uint32_t)total, 1u), (uint32_t)kMostSplits);
+        if (v.partial && kLeastSplits * total <= v.pieces) splits = (int)min((uint32_t)v.pieces / max((uint32_t)total, 1u), (uint32_t)kMostSplits);
         return (int64_t)((uint32_t)slot / (uint32_t)splits);
       });
   const int tile = slot / splits, split = slot - tile * splits;
