@@ -116,15 +116,15 @@ def attention(q, k_codes, v_codes, k_scales, v_scales, kind, page_table, kv_lens
 
 def attention_tolerance(out, lse, spread, slack, largest, positions):
     """Bounds on |out - exact| and |lse - exact| for a bf16 result of f32 sums whose weights times scales are rounded to
-    f16: half a bf16 step (2^-8) of the result, half an f16 step (2^-11) of every weight, or 2^-25 of the row's largest
-    where that is more (f16's smallest step is 2^-24, the largest is kept at 1 or above), times a code (up to 448) for
+    f16: half a bf16 step (2^-8) of the result, half an f16 step (2^-11) of every weight, or 2^-24 of the row's largest
+    where that is more (f16's smallest step is 2^-24, the largest is kept at 1/2 or above), times a code (up to 448) for
     each of `positions`; a weight is off by its score's slack
     against the maximum's (2 slack) and by the exponential (2^-21); sums of `positions` weights by their
     number of 2^-24 roundings, in the numerator and in the denominator."""
     sums = (positions + 16) * 2.0 ** -24
     # above the formula's terms stands only their product, below 2^-8 of each: the factor 1.01
     tol = 1.01 * (2.0 ** -8 * np.abs(out) + (2.0 ** -11 + 2.0 ** -20 + 2 * sums) * spread
-                  + 4 * slack[..., None] * spread + positions * 448 * 2.0 ** -25 * largest[..., None]) + 1e-37
+                  + 4 * slack[..., None] * spread + positions * 448 * 2.0 ** -24 * largest[..., None]) + 1e-37
     fine = np.where(np.isfinite(lse), np.abs(lse), 0.0)
     return tol, 1.01 * (2 * slack + sums + 2.0 ** -20 + 2.0 ** -23 * fine)
 

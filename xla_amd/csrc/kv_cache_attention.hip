@@ -211,10 +211,12 @@ __device__ __forceinline__ void columns(const uint32_t (&k)[8][N], uintx4& first
 // A weight times its value's scale goes into the matrix instruction as f16, which rounds it by 2^-11 at most; bf16 would
 // by 2^-8, as much as the result's own rounding, and the result would be 1.4 times as far from the exact one.  f16's range
 // is narrow, so a row's weights and sums carry a factor, a power of two, that keeps every scale times the factor in
-// [kLeast, kMost].  Weights are 2^8 at most (the maximum in use may lag behind by that much), so none passes 2^15, and
-// next to a row's largest one the others keep an absolute error of 2^-25 of it.  Where a scale leaves that range, the
-// weights themselves and their sum so far (`weighed`, with the factor) choose the next factor, in a branch.
-constexpr float kMost = 128.0f, kLeast = 1.0f, kLag = 8.0f;
+// [kLeast, kMost].  Weights are 2^5 at most (the maximum in use may lag behind by that much), so none passes 2^15, and
+// next to a row's largest one the others keep an absolute error of 2^-24 of it.  Where a scale leaves that range, the
+// weights themselves and their sum so far (`weighed`, with the factor) choose the next factor, in a branch.  With
+// weights of up to 2^8 and scales of up to 128 prompts whose scales have a deviation of a factor of two took 248 us for
+// 203 with equal ones; so they take 196 for 206, and 263 with a factor of four.
+constexpr float kMost = 1024.0f, kLeast = 1.0f, kLag = 5.0f;
 
 // of scales times the factor
 template <int N>
@@ -228,14 +230,18 @@ __device__ __forceinline__ bool factor_fits(const float (&x)[N]) {
   return least >= kLeast && most <= kMost;
 }
 
-// A factor is 2^-125 to 2^100, the step from one to the next at most 2^100 up.
+// A factor is 2^-123 to 2^99, the step from one to the next at most 2^100 up.
 __device__ __forceinline__ float reciprocal(float factor) { return bits_to_f32((254u << 23) - f32_to_bits(factor)); }
 
-// The factor for a row whose largest weight times scale is `most`, if not 0: their product is 32 to 64.
-__device__ __forceinline__ float new_factor(float most, float factor) {
-  const uint32_t e = min(max(f32_to_bits(most) >> 23, 32u), 254u);
-  const float now = __builtin_fminf(bits_to_f32((259u - e) << 23), factor * 0x1p100f);
-  return most > 0.0f ? now : factor;
+// The factor of a row after a step whose largest weight times scale is `weight`; `weighed` is the sum of those before,
+// with the factor.  It stays unless the weight would pass kMost or all so far is below 1/2; the larger is then 16
+// to 32, with room for later scales on both sides.
+__device__ __forceinline__ float new_factor(float weight, float weighed, float factor) {
+  const float most = __builtin_fmaxf(weight, weighed * reciprocal(factor));
+  const bool high = weight * factor > kMost;
+  if (!(high || most * factor < 0.5f) || most == 0.0f) return factor;
+  const uint32_t e = min(max(f32_to_bits(high ? weight : most) >> 23, 32u), 254u);
+  return __builtin_fminf(bits_to_f32((258u - e) << 23), factor * 0x1p100f);
 }
 
 // A scale times a new factor; finite, so that a weight of 0 cancels it.
@@ -587,12 +593,15 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
         for (int i = 0; i < 2 * S; ++i) x[i] = vs[i] * factor_v[t];
         if (__any(!factor_fits(x))) {
           KV_CACHE_RARE();
-          float weight = weighed[t] * reciprocal(factor_v[t]);
+          float weight = 0.0f, before = weighed[t];
 #pragma unroll
           for (int e = 0; e < 8; ++e) weight = __builtin_fmaxf(weight, __builtin_fabsf(y[e] * vs[(e >> 2) * S + (e & (S - 1))]));
-          weight = __builtin_fmaxf(weight, __shfl_xor(weight, 16));
-          weight = __builtin_fmaxf(weight, __shfl_xor(weight, 32));
-          const float now = new_factor(weight, factor_v[t]);
+#pragma unroll
+          for (int off = 16; off < 64; off *= 2) {
+            weight = __builtin_fmaxf(weight, __shfl_xor(weight, off));
+            before = __builtin_fmaxf(before, __shfl_xor(before, off));
+          }
+          const float now = new_factor(weight, before, factor_v[t]);
           const float step = now * reciprocal(factor_v[t]);
           factor_v[t] = now;
           weighed[t] *= step;
@@ -973,7 +982,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   // half is weighed again.
   auto catch_up = [&](int buf, auto kt_) KV_CACHE_INLINE {
     constexpr int KT = decltype(kt_)::value;
-    if (__any(more > 256.0f || !factor_fits(vq))) {
+    if (__any(more > 32.0f || !factor_fits(vq))) {
       KV_CACHE_RARE();
       float most = -INFINITY;
 #pragma unroll
@@ -983,7 +992,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
       const float scale = __builtin_amdgcn_exp2f(top - now);
       top = now;
       sum *= scale;
-      float weight = weighed * scale * reciprocal(factor_v);
+      float weight = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4 * S; ++i) vq[i] = vscale[buf][32 * KT + 8 * (i / S) + 4 * h + i % S];
 #pragma unroll
@@ -992,7 +1001,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
         weight = __builtin_fmaxf(weight, __builtin_fabsf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[KT][r], kq[i], -top)) * vq[i]));
       }
       weight = __builtin_fmaxf(weight, __shfl_xor(weight, 32));
-      const float next = new_factor(weight, factor_v);
+      const float next = new_factor(weight, __builtin_fmaxf(weighed, __shfl_xor(weighed, 32)) * scale, factor_v);
       const float step = scale * (next * reciprocal(factor_v));
       factor_v = next;
       weighed *= step;
