@@ -37,7 +37,7 @@ struct __attribute__((aligned(16))) CutTile {
 // or 32 at a time, along a range of 128-position units, 32 positions a wave; each wave has its own running
 // maximum, sum and result, which meet in LDS at the end of the range.  Per wave and 32 positions, with c = lane & 15 and
 // g = lane >> 4:
-//   S^T = K Q^T   a lane holds 16-byte pieces of key rows c straight from memory, widened to bf16 (exact for
+//   S^T = K Q^T   a lane reads 16-byte pieces of key rows c from its ring, widened to bf16 (exact for
 //                 both code types); the result has column (row of q) c and keys 4 g + i of either 16.
 //   O^T = V^T P^T the scores of a lane are, without moving, the operand's keys 4 g + i of both 16s; a lane holds
 //                 values d = 16 i + c of those eight keys, read transposed from LDS and widened to f16.
