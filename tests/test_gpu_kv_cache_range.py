@@ -1,0 +1,77 @@
+"""The calls over the 8-bit paged key/value cache at the ends of what their definition takes: caps of every size, scales
+and scores far from 1, windows and tables of 2^31 positions."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import kv_cache as plain
+from tests.test_gpu_kv_cache import KINDS, Pool, bf16, dev, offsets
+from xla_amd import ffi, ops
+
+pytestmark = pytest.mark.gpu
+
+# one row and a few heads: the streaming kernel; 64 rows of 64 heads: the prompts' kernel
+BOTH = [(1, 3), (64, 64)]
+
+
+def own_position(kind, new, group, **kw):
+    """Rows that see their own position alone (a window of 1): (got, scores, their sizes), where the log-sum-exp is the
+    row's score itself and the result the position's value.  Scores of 1e-3 to 1e3 times the usual."""
+    rng = np.random.default_rng(new + group)
+    pool = Pool(rng, kind, [new + 40], 2, 128, 64, 16)
+    pool.ks *= np.exp(rng.uniform(np.log(1e-3), np.log(1e3), pool.ks.shape)).astype(np.float32)
+    q = rng.standard_normal((new, 2 * group, 128)) * np.exp(rng.uniform(-3, 1, (new, 2 * group, 1)))
+    q[:, 0] = 0.0
+    q, qf = bf16(q)
+    scale = np.float32(kw.pop("scale", 128 ** -0.5))
+    out, lse = ops.kv_cache_attention(q, *pool.device(), dev(offsets([new])), scale=float(scale), window=1, lse=True, **kw)
+    assert ffi.last_kernel().startswith("kv_cache_attention_prompt") == (new > 1)
+    j = 40 + np.arange(new)
+    page, row = pool.table[0, j // 64], j % 64
+    k, v = (plain.values(c[page, :, row], kind).astype(np.float64) * s[page, :, row // 16].astype(np.float64)[:, :, None]
+            for c, s in ((pool.k, pool.ks), (pool.v, pool.vs)))
+    k, v = (x.repeat(group, 1) for x in (k, v))
+    got = out.float().cpu().numpy().astype(np.float64)
+    # the weight is 1, its value's scale rounded to f16 (2^-11), the result to bf16 (2^-8)
+    assert (np.abs(got - v) <= (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -20) * 1.01 * np.abs(v) + 1e-37).all()
+    x = (qf.astype(np.float64) * k).sum(-1) * float(scale)
+    return lse.cpu().numpy().astype(np.float64), x, (np.abs(qf) * np.abs(k)).sum(-1) * abs(float(scale))
+
+
+CAPS = [1e-40, 1e-6, 0.3, 3.0, 50.0, 1e3, 1e4, 1e5, 1e6, 1e7, 1e8, 1e9, 1e20, 3.3e38]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new, group", BOTH)
+@pytest.mark.parametrize("cap", CAPS)
+def test_caps_of_every_size(kind, new, group, cap):
+    """A capped score is off by its product's f32 sum (136 roundings of its size; tanh is no steeper than 1) and, relative to
+    itself, by: half the argument's way to saturation 3 * 2^-24 at most, the exponential, the sum and the reciprocal,
+    2.5 * 2^-23 of 1 - tanh, which is 1.16 tanh at most where they are used (from cap / 2 on), the polynomial below 2^-24, the
+    factors cap, log2 e and log 2 and their products 5 * 2^-24: less than 2^-20 together."""
+    got, x, size = own_position(kind, new, group, softcap=cap)
+    c = float(np.float32(cap))
+    want = c * np.tanh(x / c)
+    tol = (128 + 8) * 2.0 ** -24 * size + 2.0 ** -20 * np.abs(want) + 1e-37
+    off = np.abs(got - want)
+    assert (off <= tol).all(), ((off / tol).max(), off.max(), want.flat[(off / tol).argmax()])
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new, group", [(3, 4), (130, 32)])
+@pytest.mark.parametrize("cap", [0.5, 8.0, 1e3, 1e4, 1e6, 1e8])
+def test_attention_under_caps_of_every_size(kind, new, group, cap):
+    """Against the formula; the room that the uncapped scores have, (head + 8) 2^-24 of the product's size and more, is above
+    4 * 2^-20 of a score, so a quarter more covers the cap's 2^-20."""
+    rng = np.random.default_rng(new)
+    pool = Pool(rng, kind, [new + 300, 70], 2, 64, 32, 8)
+    q, qf = bf16(rng.standard_normal((new + 1, 2 * group, 64)) * 4)
+    off, scale = offsets([new, 1]), np.float32(64 ** -0.5)
+    out, lse = ops.kv_cache_attention(q, *pool.device(), dev(off), softcap=cap, lse=True)
+    assert ffi.last_kernel().startswith("kv_cache_attention_prompt") == (new == 130)
+    args = (qf, pool.k, pool.v, pool.ks, pool.vs, kind, pool.table, pool.lens, off, scale)
+    ref, ref_lse, spread, _, largest = plain.attention(*args, softcap=float(np.float32(cap)))
+    slack = plain.attention(*args)[3]
+    tol, tol_lse = plain.attention_tolerance(ref, ref_lse, spread, 1.25 * slack, largest, int(pool.lens.max()))
+    assert (np.abs(out.float().cpu().numpy() - ref) <= tol).all()
+    assert (np.abs(lse.cpu().numpy() - ref_lse) <= tol_lse).all()
