@@ -75,3 +75,20 @@ def test_attention_under_caps_of_every_size(kind, new, group, cap):
     tol, tol_lse = plain.attention_tolerance(ref, ref_lse, spread, 1.25 * slack, largest, int(pool.lens.max()))
     assert (np.abs(out.float().cpu().numpy() - ref) <= tol).all()
     assert (np.abs(lse.cpu().numpy() - ref_lse) <= tol_lse).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("group", [2, 64])
+@pytest.mark.parametrize("block", [16, 1])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_a_key_scale_that_is_no_number(kind, group, block, cap, bad):
+    """It reaches the result and the lse of the rows that see it, whatever the sign of their products, and no others."""
+    rng = np.random.default_rng(5)
+    pool = Pool(rng, kind, [64], 1, 128, 64, block)
+    pool.ks[pool.table[0, 0], 0, 32 // block] = bad    # positions from 32 on
+    q = rng.standard_normal((64, group, 128))
+    out, lse = ops.kv_cache_attention(bf16(q)[0], *pool.device(), dev(offsets([64])), lse=True, softcap=cap)
+    assert ffi.last_kernel().startswith("kv_cache_attention_prompt") == (group == 64)
+    assert torch.isnan(out[32:]).all() and torch.isnan(lse[32:]).all()
+    assert torch.isfinite(out[:32]).all() and torch.isfinite(lse[:32]).all()

@@ -319,13 +319,13 @@ __device__ void clear_rows_of_nobody(const AttentionView& v, int first) {
   }
 }
 
-// A value scale that is NaN or infinite moves to the score, as NaN: there it reaches the rows that see the
-// position and no others, while a weight of zero would not cancel it.
+// A scale that is NaN or infinite makes the score NaN, which reaches the rows that see the position and no others: an
+// infinite key scale would leave some of them a weight of zero or a capped score, and a weight of zero would not cancel a
+// value scale that is no number.  0 times either is NaN where it is no number, and else 0.
 __device__ __forceinline__ void keep_to_its_rows(float& key_scale, float& value_scale) {
-  if (!(__builtin_fabsf(value_scale) < INFINITY)) {
-    key_scale = bits_to_f32(0x7fc00000u);
-    value_scale = 0.0f;
-  }
+  key_scale = __builtin_fmaf(key_scale, 0.0f, key_scale);
+  key_scale = __builtin_fmaf(value_scale, 0.0f, key_scale);
+  value_scale = __builtin_fabsf(value_scale) < INFINITY ? value_scale : 0.0f;
 }
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;
