@@ -92,3 +92,15 @@ def test_a_key_scale_that_is_no_number(kind, group, block, cap, bad):
     assert ffi.last_kernel().startswith("kv_cache_attention_prompt") == (group == 64)
     assert torch.isnan(out[32:]).all() and torch.isnan(lse[32:]).all()
     assert torch.isfinite(out[:32]).all() and torch.isfinite(lse[:32]).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new, group", BOTH)
+@pytest.mark.parametrize("scale", [-1e32, 1e30, 1e34])
+def test_scores_of_every_size(kind, new, group, scale):
+    """Scores far below -1e30 are scores: the row's sum is 1 and its lse the score, off by the product's f32 sum and, relative
+    to itself, the scale, log2 e, log 2 and their products."""
+    got, x, size = own_position(kind, new, group, scale=scale)
+    assert (x < -1e31).any()
+    tol = (128 + 8) * 2.0 ** -24 * size + 6 * 2.0 ** -24 * np.abs(x)
+    assert (np.abs(got - x) <= tol).all()

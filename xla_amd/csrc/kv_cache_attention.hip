@@ -209,6 +209,9 @@ __device__ __forceinline__ void columns(const uint32_t (&k)[8][N], uintx4& first
   }
 }
 
+// A row's maximum before any score: below every other number, and finite, so that a difference to it is no NaN.
+constexpr float kNoScore = -0x1.fffffep127f;
+
 // A weight times its value's scale goes into the matrix instruction as f16, which rounds it by 2^-11 at most; bf16 would
 // by 2^-8, as much as the result's own rounding, and the result would be 1.4 times as far from the exact one.  f16's range
 // is narrow, so a row's weights and sums carry a factor, a power of two, that keeps every scale times the factor in
@@ -518,7 +521,7 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
     float top[QT], sum[QT], factor_v[QT], weighed[QT];
 #pragma unroll
     for (int t = 0; t < QT; ++t) {
-      top[t] = -1e30f;  // below every score, and finite
+      top[t] = kNoScore;
       factor_v[t] = 1.0f;
       weighed[t] = 0.0f;
       sum[t] = 0.0f;
@@ -849,7 +852,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     sees_lo = v.a.window > 0 ? max(0, p - v.a.window + 1) : 0;
   }
   floatx16 acc[DP / 32];
-  float top = -1e30f, sum = 0.0f, factor_v = 1.0f, weighed = 0.0f;
+  float top = kNoScore, sum = 0.0f, factor_v = 1.0f, weighed = 0.0f;
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i)
 #pragma unroll
@@ -1174,7 +1177,7 @@ __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(JoinView v
   auto piece = [&](int w) { return first + (w * p.piece_step - (w > 0 ? p.back : 0)); };
   const int64_t tops = (int64_t)p.tile_rows * size + r;
   const int d = min(4 * lane, size - 4);
-  float m = -1e30f, l = 0.0f;
+  float m = kNoScore, l = 0.0f;
   floatx4 o = {0.0f, 0.0f, 0.0f, 0.0f};
   for (int w0 = 0; w0 < cut.pieces; w0 += L) {
     const int here = min(cut.pieces - w0, L);
