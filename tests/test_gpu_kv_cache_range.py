@@ -107,3 +107,29 @@ def test_scores_of_every_size(kind, new, group, scale):
     assert (x < -1e31).any()
     tol = (128 + 8) * 2.0 ** -24 * size + 6 * 2.0 ** -24 * np.abs(x)
     assert (np.abs(got - x) <= tol).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("new, group", BOTH)
+@pytest.mark.parametrize("scale", [1.0, 1e6, 1e9, 1e12, 1e30])
+def test_one_score_far_above_the_others(kind, new, group, scale):
+    """Position 77's product is 2 q . 112 / 3 and the others' are below q . 112 / 3 at most, q being 1 or more: all
+    weights but one are below e^-37, however large the scores are, and the result is that position's value."""
+    rng = np.random.default_rng(9)
+    pool = Pool(rng, kind, [400 + new], 2, 64, 64, 16)
+    pool.k[:] = 0
+    pool.ks[:] = 1 / 3
+    pool.k[..., 0] = rng.integers(-112, 113, pool.k.shape[:3]) if kind == "s8" else rng.integers(0, 0x6e, pool.k.shape[:3])
+    pool.k[pool.table[0, 1], :, 13, :2] = 112 if kind == "s8" else 0x6e    # 77; 112 either way
+    q = np.zeros((new, 2 * group, 64))
+    q[..., :2] = np.abs(rng.standard_normal((new, 2 * group, 1))) + 1
+    q, qf = bf16(q)
+    out, lse = ops.kv_cache_attention(q, *pool.device(), dev(offsets([new])), scale=scale, lse=True)
+    assert ffi.last_kernel().startswith("kv_cache_attention_prompt") == (new > 1)
+    v = plain.values(pool.v[pool.table[0, 1], :, 13], kind) * pool.vs[pool.table[0, 1], :, 0][:, None]
+    v = v.repeat(group, 0)[None].astype(np.float64)
+    got = out.float().cpu().numpy()
+    # an f16 weight, a bf16 result, 464 weights of e^-37 times values up to 1.5 * 448 / 110
+    assert (np.abs(got - v) <= (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -20) * 1.01 * np.abs(v) + 1e-12).all()
+    x = 2 * qf[..., 0].astype(np.float64) * 112 * float(np.float32(1 / 3)) * float(np.float32(scale))
+    assert (np.abs(lse.cpu().numpy() - x) <= 8 * 2.0 ** -24 * x).all()

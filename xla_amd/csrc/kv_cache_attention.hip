@@ -1012,14 +1012,20 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     p[KT][I >> 1] = __builtin_bit_cast(halfx8, packed);
   };
   // Where the weights' sum shows that the maximum in use lags too far behind, or a scale leaves the factor's range, the
-  // half is weighed again.
+  // half is weighed again, on scores that are products rounded as the maximum is: the unrounded ones that it was weighed on
+  // first may lie beside it by 2^-24 of themselves, which from scores of 2^27 on is more than a weight bears.
   auto catch_up = [&](int buf, auto kt_) KV_CACHE_INLINE {
     constexpr int KT = decltype(kt_)::value;
     if (__any(more > 32.0f || !factor_fits(vq))) {
       KV_CACHE_RARE();
       float most = -INFINITY;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) most = __builtin_fmaxf(most, sc[KT][r] * kq[(r >> 2) * S + (r & (S - 1))]);
+      for (int r = 0; r < 16; ++r) {
+        sc[KT][r] *= kq[(r >> 2) * S + (r & (S - 1))];
+        most = __builtin_fmaxf(most, sc[KT][r]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4 * S; ++i) kq[i] = 1.0f;
       most = __builtin_fmaxf(most, __shfl_xor(most, 32));
       const float now = __builtin_fmaxf(top, most);
       const float scale = __builtin_amdgcn_exp2f(top - now);
@@ -1031,7 +1037,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int i = (r >> 2) * S + (r & (S - 1));
-        weight = __builtin_fmaxf(weight, __builtin_fabsf(__builtin_amdgcn_exp2f(__builtin_fmaf(sc[KT][r], kq[i], -top)) * vq[i]));
+        weight = __builtin_fmaxf(weight, __builtin_fabsf(__builtin_amdgcn_exp2f(sc[KT][r] - top) * vq[i]));
       }
       weight = __builtin_fmaxf(weight, __shfl_xor(weight, 32));
       const float next = new_factor(weight, __builtin_fmaxf(weighed, __shfl_xor(weighed, 32)) * scale, factor_v);
