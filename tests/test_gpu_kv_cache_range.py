@@ -133,3 +133,32 @@ def test_one_score_far_above_the_others(kind, new, group, scale):
     assert (np.abs(got - v) <= (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -20) * 1.01 * np.abs(v) + 1e-12).all()
     x = 2 * qf[..., 0].astype(np.float64) * 112 * float(np.float32(1 / 3)) * float(np.float32(scale))
     assert (np.abs(lse.cpu().numpy() - x) <= 8 * 2.0 ** -24 * x).all()
+
+
+@pytest.mark.parametrize("group", [1, 4])
+def test_a_window_of_nearly_all_positions(group):
+    """A table of 2^31 - 1040 positions and a window just below, more rows than positions: the first rows stand 5000 before
+    the sequence, and such a position less the window does not fit 32 bits."""
+    rng = np.random.default_rng(13)
+    new, length, window = 6000, 1000, 2 ** 31 - 1045
+    pool = Pool(rng, "s8", [length], 1, 16, 16, 16)
+    tensors = pool.device()
+    tensors[4] = torch.full((1, 2 ** 27 - 65), -1, dtype=torch.int32, device="cuda")
+    tensors[4][:, :pool.table.shape[1]] = dev(pool.table)
+    q, qf = bf16(rng.standard_normal((new, group, 16)))
+    for scratch in ("auto", None):
+        out, lse = ops.kv_cache_attention(q, *tensors, dev(offsets([new])), window=window, lse=True, scratch=scratch)
+        assert ffi.last_kernel().startswith("kv_cache_attention_prompt")
+        ref, ref_lse, spread, slack, largest = plain.attention(qf, pool.k, pool.v, pool.ks, pool.vs, "s8", pool.table, pool.lens,
+                                                               offsets([new]), np.float32(0.25), window=window)
+        tol, tol_lse = plain.attention_tolerance(ref, ref_lse, spread, slack, largest, length)
+        assert (np.abs(out.float().cpu().numpy() - ref) <= tol).all()
+        got = lse.cpu().numpy()
+        assert np.isneginf(got[:5000]).all() and (np.abs(got[5000:] - ref_lse[5000:]) <= tol_lse[5000:]).all()
+    # few rows for the streaming kernel, 1490 of them in front of the sequence
+    out = ops.kv_cache_attention(q[:1500, :1].contiguous(), *tensors[:5], dev(np.array([10], np.int32)), dev(offsets([1500])), window=window)
+    assert not ffi.last_kernel().startswith("kv_cache_attention_prompt")
+    ref, ref_lse, spread, slack, largest = plain.attention(qf[:1500, :1], pool.k, pool.v, pool.ks, pool.vs, "s8", pool.table, [10],
+                                                           offsets([1500]), np.float32(0.25), window=window)
+    tol, _ = plain.attention_tolerance(ref, ref_lse, spread, slack, largest, 10)
+    assert (np.abs(out.float().cpu().numpy() - ref) <= tol).all() and ref[-10:].all()

@@ -24,6 +24,12 @@ struct AttentionView {
   int causal, window;
 };
 
+// The first position that the row at position p sees.  A row in front of its sequence (p < 0) sees none; its p less a
+// window of nearly 2^31 would leave 32 bits.
+static __device__ __forceinline__ int window_start(const AttentionView& v, int p) {
+  return v.window > 0 ? max(0, max(p, 0) - v.window + 1) : 0;
+}
+
 // A tile of packed rows whose positions several workgroups share.
 struct __attribute__((aligned(16))) CutTile {
   int row0;    // the sequence's first row
@@ -77,7 +83,7 @@ __device__ __forceinline__ DecodeSpan decode_span(const DecodeView& v, int b) {
   DecodeSpan r;
   r.s = kv_sequence(v.a.c, b);
   const int rows = r.s.n * v.a.group;
-  r.lo = v.a.window > 0 ? max(0, r.s.len - r.s.n - v.a.window + 1) : 0;
+  r.lo = window_start(v.a, r.s.len - r.s.n);
   r.hi = r.s.len;
   const bool mine = rows > v.rows_from && rows <= v.rows_to;
   r.tiles = mine ? (rows + RT - 1) / RT : 0;
@@ -496,10 +502,10 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
       }
       const int p = sp.s.len - sp.s.n + i;
       sees_hi[t] = v.a.causal ? min(sp.hi, p + 1) : sp.hi;
-      sees_lo[t] = v.a.window > 0 ? max(0, p - v.a.window + 1) : 0;
+      sees_lo[t] = window_start(v.a, p);
     }
     if (v.a.causal) all_hi = min(all_hi, sp.s.len - sp.s.n + r0 / v.a.group + 1);
-    if (v.a.window > 0) all_lo = max(0, sp.s.len - sp.s.n + (r0 + rows - 1) / v.a.group - v.a.window + 1);
+    if (v.a.window > 0) all_lo = window_start(v.a, sp.s.len - sp.s.n + (r0 + rows - 1) / v.a.group);
 
     // q is here before the loop's loads are counted
 #pragma unroll
@@ -828,9 +834,9 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
   const int r0 = __builtin_amdgcn_readfirstlane((int)(tile - spot.before)) * RT, rows = min(s.n * v.a.group - r0, RT);
   const int p_first = s.len - s.n + r0 / v.a.group, p_last = s.len - s.n + (r0 + rows - 1) / v.a.group;
   // positions that some row of the tile sees, and that all of them see
-  const int lo = v.a.window > 0 ? max(0, p_first - v.a.window + 1) : 0;
+  const int lo = window_start(v.a, p_first);
   const int hi = v.a.causal ? min(s.len, p_last + 1) : s.len;
-  const int all_lo = v.a.window > 0 ? max(0, p_last - v.a.window + 1) : 0;
+  const int all_lo = window_start(v.a, p_last);
   const int all_hi = v.a.causal ? min(s.len, p_first + 1) : s.len;
   const int u_first = lo / kStage, u_count = max((hi + kStage - 1) / kStage - u_first, 0);
   splits = min(splits, max(u_count / kLeastStages, 1));
@@ -849,7 +855,7 @@ __global__ __launch_bounds__(256, DP <= 128 ? 2 : 1) void kv_cache_attention_pro
     for (int k = 0; k < DP / 16; ++k) q[k] = 16 * k < c.head ? *reinterpret_cast<const bf16x8*>(qr + 16 * k + 8 * h) : bf16x8{};
     const int p = s.len - s.n + i;
     sees_hi = v.a.causal ? min(s.len, p + 1) : s.len;
-    sees_lo = v.a.window > 0 ? max(0, p - v.a.window + 1) : 0;
+    sees_lo = window_start(v.a, p);
   }
   floatx16 acc[DP / 32];
   float top = kNoScore, sum = 0.0f, factor_v = 1.0f, weighed = 0.0f;
