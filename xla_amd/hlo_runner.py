@@ -54,6 +54,30 @@ def parse_backend_config(cfg):
     return out
 
 
+def _aliased(ins):
+    """{result: operand} of an instruction's output_to_operand_aliasing."""
+    return {int(m.group(1) or 0): int(m.group(2)) for m in
+            re.finditer(r"\{(\d*)\}:\s*\((\d+),", ins["attrs"].get("output_to_operand_aliasing", ""))}
+
+
+def still_read(instructions, at, env, operands, i):
+    """Whether the buffer of operand i of instruction `at` is read beside it: by another operand of the same instruction, by a
+    later instruction through a value of `env` that holds it, or by the caller, as the root's."""
+    t = operands[i]
+    if any(x is t for k, x in enumerate(operands) if k != i):
+        return True
+
+    def holds(name, index=None):
+        v = env.get(name)
+        if isinstance(v, (list, tuple)):
+            return any(x is t for x in (v if index is None else [v[index]]))
+        return v is t
+    if any(ins["root"] and holds(ins["name"]) for ins in instructions[:at]):
+        return True
+    return any(holds(o, int(ins["attrs"]["index"]) if ins["opcode"] == "get-tuple-element" else None)
+               for ins in instructions[at + 1:] for o in ins["operands"])
+
+
 class Executable:
     """A rewritten module bound to the registry of an FFI host."""
 
@@ -78,12 +102,16 @@ class Executable:
         root value (a list for a tuple)."""
         env, shapes = {}, {}
         self.host.stream = torch.cuda.current_stream().cuda_stream
-        for ins in self.entry["instructions"]:
+        for at, ins in enumerate(self.entry["instructions"]):
             op, sh = ins["opcode"], ins["shape"]
             x = [env[o] for o in ins["operands"]]
             if op == "parameter":
                 v = args[int(ins["literal"])]
             elif op == "custom-call":
+                for i in sorted(set(_aliased(ins).values())):
+                    # the call writes over its operand: a value that is still read is left as it is, as XLA's copy insertion does
+                    if still_read(self.entry["instructions"], at, env, x, i):
+                        x[i] = x[i].clone()
                 v = self._call(ins, x, [shapes[o] for o in ins["operands"]])
             elif op == "get-tuple-element":
                 v = x[0][int(ins["attrs"]["index"])]
@@ -119,9 +147,7 @@ class Executable:
         if ins["attrs"].get("api_version") != "API_VERSION_TYPED_FFI":
             raise ValueError("custom call %s does not use the typed FFI" % ins["name"])
         res_shapes = ins["shape"]["tuple"] if "tuple" in ins["shape"] else [ins["shape"]]
-        # a result that the instruction aliases with an operand is that operand's buffer
-        alias = {int(m.group(1) or 0): int(m.group(2)) for m in
-                 re.finditer(r"\{(\d*)\}:\s*\((\d+),", ins["attrs"].get("output_to_operand_aliasing", ""))}
+        alias = _aliased(ins)  # a result that the instruction aliases with an operand is that operand's buffer
         results = [operands[alias[i]] if i in alias else torch.empty(s["dims"], dtype=_TORCH[s["dtype"]], device="cuda")
                    for i, s in enumerate(res_shapes)]
         args = [(_DT[s["dtype"]], t.data_ptr(), s["dims"]) for t, s in zip(operands, operand_shapes)]
