@@ -212,7 +212,8 @@ XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_kv_cache_pages(XLA_FFI_CallFrame* call_fra
  * Copies whole pages inside every buffer of a pool: for each (source, destination) of moves,
  * buffer[destination] = buffer[source].  Pairs that name a page outside [0, pages) are skipped.  No
  * destination may occur twice or be a source too.
- *   args: moves S32 [m, 2]; 1 to XLA_AMD_KV_CACHE_MAX_BUFFERS buffers of any type [pages, ...]
+ *   args: moves S32 [m, 2]; 1 to XLA_AMD_KV_CACHE_MAX_BUFFERS buffers [pages, ...] of any type whose values fill
+ *         whole bytes
  *   rets: the buffers, the operands' own (output_to_operand_aliasing)
  */
 XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_kv_cache_copy_pages(XLA_FFI_CallFrame* call_frame);

@@ -337,12 +337,17 @@ bool SameShape(const XLA_FFI_Buffer* a, const XLA_FFI_Buffer* b) {
 // Types whose values fill whole bytes, and how many.
 constexpr uint64_t kWholeByteMask =
     Bit(XLA_FFI_DataType_PRED) | Bit(XLA_FFI_DataType_S8) | Bit(XLA_FFI_DataType_U8) | Bit(XLA_FFI_DataType_F8E4M3FN) |
-    Bit(XLA_FFI_DataType_F8E5M2) | Bit(XLA_FFI_DataType_S16) | Bit(XLA_FFI_DataType_U16) | Bit(XLA_FFI_DataType_F16) |
-    Bit(XLA_FFI_DataType_BF16) | Bit(XLA_FFI_DataType_S32) | Bit(XLA_FFI_DataType_U32) | Bit(XLA_FFI_DataType_F32);
+    Bit(XLA_FFI_DataType_F8E5M2) | Bit(XLA_FFI_DataType_F8E4M3B11FNUZ) | Bit(XLA_FFI_DataType_F8E5M2FNUZ) |
+    Bit(XLA_FFI_DataType_F8E4M3FNUZ) | Bit(XLA_FFI_DataType_F8E4M3) | Bit(XLA_FFI_DataType_F8E3M4) | Bit(XLA_FFI_DataType_F8E8M0FNU) |
+    Bit(XLA_FFI_DataType_S16) | Bit(XLA_FFI_DataType_U16) | Bit(XLA_FFI_DataType_F16) | Bit(XLA_FFI_DataType_BF16) |
+    Bit(XLA_FFI_DataType_S32) | Bit(XLA_FFI_DataType_U32) | Bit(XLA_FFI_DataType_F32) | Bit(XLA_FFI_DataType_S64) |
+    Bit(XLA_FFI_DataType_U64) | Bit(XLA_FFI_DataType_F64) | Bit(XLA_FFI_DataType_C64) | Bit(XLA_FFI_DataType_C128);
 int64_t ElementBytes(int d) {
   switch (d) {
     case XLA_FFI_DataType_S16: case XLA_FFI_DataType_U16: case XLA_FFI_DataType_F16: case XLA_FFI_DataType_BF16: return 2;
     case XLA_FFI_DataType_S32: case XLA_FFI_DataType_U32: case XLA_FFI_DataType_F32: return 4;
+    case XLA_FFI_DataType_S64: case XLA_FFI_DataType_U64: case XLA_FFI_DataType_F64: case XLA_FFI_DataType_C64: return 8;
+    case XLA_FFI_DataType_C128: return 16;
     default: return 1;
   }
 }

@@ -17,6 +17,7 @@ U8, U16, U32, U64 = 6, 7, 8, 9
 F16, F32, F64, BF16 = 10, 11, 12, 16
 F8E5M2, F8E4M3FN, S4, U4 = 19, 20, 21, 22
 F8E8M0FNU = 33
+C64, C128, F8E4M3B11FNUZ, F8E5M2FNUZ, F8E4M3FNUZ, F8E4M3, F8E3M4 = 15, 18, 23, 24, 25, 28, 29  # moved, never computed with
 
 DTYPE_NAMES = {PRED: "PRED", S8: "S8", S16: "S16", S32: "S32", S64: "S64", U8: "U8", U16: "U16",
                U32: "U32", U64: "U64", F16: "F16", F32: "F32", F64: "F64", BF16: "BF16",

@@ -197,7 +197,10 @@ def rowwise_quantize_fp8(x, gamma=None, *, eps=1e-6, q=None, scales=None, build_
 _CACHE = {torch.int8: dtypes.S8, torch.float8_e4m3fn: dtypes.F8E4M3FN, torch.uint8: dtypes.F8E4M3FN}
 _ANY = {torch.int8: dtypes.S8, torch.uint8: dtypes.U8, torch.float8_e4m3fn: dtypes.F8E4M3FN, torch.bool: dtypes.PRED,
         torch.float8_e5m2: dtypes.F8E5M2, torch.bfloat16: dtypes.BF16, torch.float16: dtypes.F16, torch.int16: dtypes.S16,
-        torch.float32: dtypes.F32, torch.int32: dtypes.S32}
+        torch.float32: dtypes.F32, torch.int32: dtypes.S32, torch.uint16: dtypes.U16, torch.uint32: dtypes.U32,
+        torch.float8_e8m0fnu: dtypes.F8E8M0FNU, torch.float8_e5m2fnuz: dtypes.F8E5M2FNUZ,
+        torch.float8_e4m3fnuz: dtypes.F8E4M3FNUZ, torch.int64: dtypes.S64, torch.uint64: dtypes.U64, torch.float64: dtypes.F64,
+        torch.complex64: dtypes.C64, torch.complex128: dtypes.C128}
 
 
 def _operand(t, name, kinds, rank=None):
@@ -342,7 +345,7 @@ def kv_cache_pages(op, page_table, kv_lens, ref_counts, request=None, *, page_si
 
 def kv_cache_copy_pages(moves, buffers, *, build_only=False):
     """buffer[destination] = buffer[source] for every (source, destination) of moves (int32 [m, 2]) in every one of
-    `buffers` ([pages, ...], up to 64), in place; returns the buffers.  Pairs that name a page outside the pool
+    `buffers` ([pages, ...] of any type, up to 64), in place; returns the buffers.  Pairs that name a page outside the pool
     (as the -1 behind the moves of kv_cache_pages) are skipped; no destination may occur twice or be a source."""
     buffers = list(buffers)
     device = _one_device(moves, *buffers)
