@@ -169,7 +169,8 @@ XLA_AMD_EXPORT XLA_FFI_Error* xla_amd_kv_cache_write(XLA_FFI_CallFrame* call_fra
  *   out = sum_j exp(x_j) v_j / sum_j exp(x_j);  lse = log sum_j exp(x_j)
  *   A row that sees nothing, or belongs to nobody, is 0 and its lse -infinity.
  *   Sums, maxima and the softmax are f32; the weights exp(x_j) times the scale of v_j are rounded to f16 on their way
- *   into the matrix instruction, next to the row's largest one: by 2^-11 of each, or 2^-24 of the largest if that is more.
+ *   into the matrix instruction: by 2^-11 of each, or 2^-24 of the sum of their magnitudes over the row if that is more.
+ *   A capped score is off by 2^-20 of itself at most, whatever the cap, besides its product's f32 sum.
  *   A row that sees a key's or a value's scale that is NaN or infinite is NaN, its lse too; no other row is.
  *   At most 2^29 rows times heads.
  *   args: q BF16 [rows, q_heads, head]; k_cache, v_cache, k_scales, v_scales, page_table, kv_lens, q_offsets

@@ -58,9 +58,9 @@ struct __attribute__((aligned(16))) CutTile {
 // scratch, at most two for each worker, and a second launch joins them in order.  The worker in whose range a cut
 // tile begins notes where its pieces are, so the second launch looks for nothing.
 //
-// Bound: HBM, 2 (head + 4 / block) bytes for each position and cache head.  64 sequences of up to 8192 positions, 8 heads
-// of 128: 110 us, 4.9 TB/s, where 512 workgroups that read pages of 64 KB in any order reach 6.1 and a linear read 7.05;
-// four sequences of 131072: 186 us, 5.3 TB/s.  The same call on pages that stay in the caches takes 75 to 79 us.
+// Bound: HBM, 2 (head + 4 / block) bytes for each position and cache head.  64 sequences of up to 8192 positions, 32 heads
+// on 8 of 128, s8: 110 us, 4.9 TB/s, where a linear read reaches 7.05; four sequences of 131072, 64 heads on 8, f8: 185 us,
+// 5.4 TB/s.  With tables that name 64 pages again and again, which stay in the caches, they take 80 and 123 us.
 constexpr int kUnit = 128;
 
 struct DecodeView {
@@ -222,10 +222,10 @@ constexpr float kNoScore = -0x1.fffffep127f;
 // by 2^-8, as much as the result's own rounding, and the result would be 1.4 times as far from the exact one.  f16's range
 // is narrow, so a row's weights and sums carry a factor, a power of two, that keeps every scale times the factor in
 // [kLeast, kMost].  Weights are 2^5 at most (the maximum in use may lag behind by that much), so none passes 2^15, and
-// next to a row's largest one the others keep an absolute error of 2^-24 of it.  Where a scale leaves that range, the
-// weights themselves and their sum so far (`weighed`, with the factor) choose the next factor, in a branch.  With
-// weights of up to 2^8 and scales of up to 128 prompts whose scales have a deviation of a factor of two took 248 us for
-// 203 with equal ones; so they take 196 for 206, and 263 with a factor of four.
+// the row's sum times the factor stays at 1/2 or above, so the smallest keep an absolute error of 2^-24 of the sum.  Where a
+// scale leaves that range, the weights themselves and their sum so far (`weighed`, with the factor) choose the next
+// factor, in a branch.  A prompt of 4096 rows, 32 heads on 8 of 128, whose value scales deviate by a factor of two takes 191
+// us, one with equal scales 205, by a factor of four 256.
 constexpr float kMost = 1024.0f, kLeast = 1.0f, kLag = 5.0f;
 
 // of scales times the factor
@@ -771,14 +771,16 @@ __global__ __launch_bounds__(256, decode_residents(DP)) void kv_cache_attention_
 //
 // Bound: two waves share a SIMD, and each needs 1400 cycles of vector instructions (a quarter of them exponentials) and
 // 1024 of matrix instructions for a stage of a head of 128, the matrix pipes being busy for 38% of the time.  8192 rows of
-// 32 heads on 8192 positions, causal: 635 us, 866 TFLOP/s, where a large product of matrices reaches 1357.
+// 32 heads on 8192 positions, causal: 630 to 670 us from run to run, 820 to 870 TFLOP/s, where a large product of matrices
+// reaches 1357.
 constexpr int kStage = 64;
 constexpr int kPromptRows = 128;
 // Where a call has few tiles, their positions are cut: into pieces that give kPieces workgroups at most (six chunks of
-// prompts, 312 tiles and heads: 82 us with 512, which cuts none, 73 with 768, 67 with 1024, 83 with 1536), kLeastSplits to
-// kMostSplits for a tile, of kLeastStages stages or more.  512 workgroups run at a time, so tiles that fill them once
-// stay whole: 4 chunks of 512 rows on 4096 positions (512 tiles and heads) take 199 us whole and 232 cut in two, two
-// prompts of 1024 64 and 79.  How many tiles there are is device data, so each workgroup counts them.
+// prompts, 312 tiles and heads: 127 us with 512, which cuts none, 76 with 768 and two pieces a tile, 70 with 1024, 84 with
+// 1536), kLeastSplits to kMostSplits for a tile, of kLeastStages stages or more.  512 workgroups run at a time, so tiles
+// that fill them once stay whole: 4 chunks of 512 rows on 4096 positions (512 tiles and heads) take 179 us whole and 199
+// cut in two, two prompts of 1024 65 and 73; from 342 tiles and heads on, where three pieces each would be too many, part
+// of the device has nothing to do.  How many tiles there are is device data, so each workgroup counts them.
 constexpr int kPieces = 1024;
 constexpr int kLeastSplits = 3;
 constexpr int kMostSplits = 16;
@@ -1175,7 +1177,7 @@ struct JoinView {
 
 // L lanes for a row, four values each; the pieces in their order.  The maxima and sums of up to L pieces are a lane's
 // each, and the results are under way four pieces at a time.
-// Bound: three dependent reads (the tile's note, the maxima, the results): 4.4 us for one sequence's 64 rows, 4.9 for 64.
+// Bound: three dependent reads (the tile's note, the maxima, the results): 4.2 us for one sequence, 5.0 for 64.
 template <int L>
 __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(JoinView v) {
   const JoinPart& p = blockIdx.x < v.blocks ? v.parts[0] : v.parts[1];
@@ -1223,12 +1225,15 @@ __global__ __launch_bounds__(256) void kv_cache_attention_join_kernel(JoinView v
 }
 
 // Packed rows of a sequence up to which the streaming kernel takes it in calls that both kernels serve, two of its
-// tiles: 64 sequences of 64 packed rows on 4096 positions take 217 us there and 241 in the other, of 68 320 and 248.
+// tiles: 64 sequences on 4096 positions take 201 us there and 202 in the other with 36 packed rows each, 214 and 182 with
+// 48, 217 and 179 with 64, and with 68, a third tile, 310 and 188; with 64 on 1024 positions 64 in either.
 constexpr int kFewRows = 64;
 // Packed rows beyond one row for each sequence up to which the streaming kernel takes a whole call, since two
 // kernels one after the other each have an end at which little runs.  32 heads on 8 of 128, streaming alone and both:
-// 63 single rows and one chunk of 512 on 4096 positions (2044 to spare) 167 and 187 us, a prompt of 512 25 and 40;
-// 64 x 17 rows on 4096 (4096 to spare) 308 and 222, a prompt of 2048 (8188) 168 and 93.
+// 63 single rows and one chunk of 512 on 4096 positions (2044 to spare) 140 and 172 us, a prompt of 512 22 and 36;
+// 64 x 17 rows on 4096 (4096 to spare) 304 and 188, a prompt of 2048 (8188) 192 and 90.  Shapes alone are known here: a
+// sequence without rows counts as one with a row, so a table of more slots than the call uses leaves a prompt of up to
+// that many rows more with the streaming kernel, and rows of nobody count as rows to spare.
 constexpr int kSpareRows = 2048;
 
 // How a call runs, from its shapes alone (lengths are device data).
@@ -1255,8 +1260,8 @@ DecodePlan PlanDecode(int64_t rows, int64_t batch, int64_t q_heads, int64_t kv_h
   if (w > units) w = units;
   d.workers = w < 1 ? 1 : (int)w;
   // A second launch costs more than four units one after the other (two of a head above 128).  Eight heads of 128, cut and
-  // whole: one sequence of 500 positions 10.4 and 10.1 us, of 760 11.0 and 12.3; eight 12.3 and 10.5, 12.9 and 16.0;
-  // 64 of 500 19.8 and 17.9.  A head of 256: one of 250 12.9 and 11.0, of 500 12.9 and 14.9.
+  // whole: one sequence of 500 positions 10.6 and 9.8 us, of 760 11.3 and 11.5; eight 12.4 and 10.1, 13.0 and 14.3;
+  // 64 of 500 19.3 and 17.2.  A head of 256: one of 250 13.2 and 10.8, of 500 13.0 and 13.7.
   d.split = positions > (d.dp == 256 ? 2 : 4) * kUnit && batch > 0;
   d.bytes = d.split ? (size_t)(d.workers * (sizeof(CutTile) + kv_heads * 2 * 16 * d.qt * (head + 2) * 4)) : 0;
   return d;
