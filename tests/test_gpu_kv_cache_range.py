@@ -49,7 +49,7 @@ CAPS = [1e-40, 1e-6, 0.3, 3.0, 50.0, 1e3, 1e4, 1e5, 1e6, 1e7, 1e8, 1e9, 1e20, 3.
 @pytest.mark.parametrize("cap", CAPS)
 def test_caps_of_every_size(kind, new, group, cap):
     """A capped score is off by its product's f32 sum (136 roundings of its size; tanh is no steeper than 1) and, relative to
-    itself, by: half the argument's way to saturation 3 * 2^-24 at most, the exponential, the sum and the reciprocal,
+    itself, by: the argument's three roundings, 3 * 2^-24 at most, the exponential, the sum and the reciprocal,
     2.5 * 2^-23 of 1 - tanh, which is 1.16 tanh at most where they are used (from cap / 2 on), the polynomial below 2^-24, the
     factors cap, log2 e and log 2 and their products 5 * 2^-24: less than 2^-20 together."""
     got, x, size = own_position(kind, new, group, softcap=cap)

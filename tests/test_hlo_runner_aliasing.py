@@ -43,6 +43,17 @@ def test_what_is_still_read(root):
     assert hlo_runner.still_read(entry, at["first"], env, [moves, a, a], 1)
 
 
+def test_a_tuple_in_a_tuple():
+    text = MODULE.replace("  second =", "  nest = ((s8[4,16], f32[4,3]), s32[1,2]) tuple(first, more)\n  second =")
+    for root, want in (("inner = (s8[4,16], f32[4,3]) get-tuple-element(nest), index=0\n  ROOT r = (s8[4,16], (s8[4,16], f32[4,3])) tuple(second, inner)", True),
+                       ("m = s32[1,2] get-tuple-element(nest), index=1\n  ROOT r = (s8[4,16], s32[1,2]) tuple(second, m)", False)):
+        entry = next(c for c in hlo.to_json(text % root)["computations"] if c["entry"])["instructions"]
+        at = [i["name"] for i in entry].index("second")
+        a1, b1, more = object(), object(), object()
+        env = {"first": [a1, b1], "a1": a1, "more": more, "nest": [[a1, b1], more]}
+        assert hlo_runner.still_read(entry, at, env, [more, a1], 1) == want
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("root", ROOTS)
 def test_a_module_that_reads_what_a_call_has_written_over(root):

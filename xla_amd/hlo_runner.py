@@ -67,11 +67,12 @@ def still_read(instructions, at, env, operands, i):
     if any(x is t for k, x in enumerate(operands) if k != i):
         return True
 
+    def inside(v):
+        return any(inside(x) for x in v) if isinstance(v, (list, tuple)) else v is t
+
     def holds(name, index=None):
         v = env.get(name)
-        if isinstance(v, (list, tuple)):
-            return any(x is t for x in (v if index is None else [v[index]]))
-        return v is t
+        return inside(v[index] if index is not None and isinstance(v, (list, tuple)) else v)
     if any(ins["root"] and holds(ins["name"]) for ins in instructions[:at]):
         return True
     return any(holds(o, int(ins["attrs"]["index"]) if ins["opcode"] == "get-tuple-element" else None)
